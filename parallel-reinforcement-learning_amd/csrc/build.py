@@ -25,7 +25,10 @@ LIB = os.path.join(PKG, "libprl_hip.so")
 OBJDIR = os.path.join(HERE, "build")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CFLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-ffp-contract=off",
-          "-fno-gpu-rdc", "-Wall", "-Wno-unused-function", "-Wno-unused-variable"]
+          "-fno-gpu-rdc", "-Wall", "-Wno-unused-function", "-Wno-unused-variable",
+          # no packed FP32 instructions (v_pk_add / mul / fma_f32, which -O3 forms from ordinary
+          # float code): some of their forms have given wrong results now and then on MI355X
+          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 STAMPED = "prl_abi.hip"   # the translation unit that carries the source stamp
 
 
