@@ -32,6 +32,7 @@ import prl_native
 from .ActorCritic import ActorCritic
 from .Memory import Memory
 from .RND import RND
+from .optim import AdamW, clip_and_step
 
 device = torch.device("cuda" if torch.cuda.is_available() else "cpu")
 
@@ -376,7 +377,10 @@ class PPO:
         self.policy_old.load_state_dict(self.policy.state_dict())
 
     def _fused_engine(self):
-        """The fused update engine for this policy / mini_batch (None: shape outside it)."""
+        """The fused update engine for this policy / mini_batch (None: shape outside it, or an
+        optimizer whose state the engine does not hold: optim.AdamW with 8-bit moments)."""
+        if isinstance(self.optimizer, AdamW) and not self.optimizer.flat_state():
+            return None
         eng = getattr(self, "_engine", None)
         if eng is not None and eng.mini_batch == self.mini_batch_size:
             return eng
@@ -485,8 +489,7 @@ class PPO:
             (loss * ((hi - lo) / count_j) if world > 1 else loss).backward()
         if flat is not None:
             self.all_reduce(flat)
-        nn.utils.clip_grad_norm_(params, 2.0)
-        self.optimizer.step()
+        clip_and_step(self.optimizer, params, 2.0)
         return loss
 
     def load_weights(self, path: str):  # PPO.py:262-277

@@ -18,9 +18,10 @@ from __future__ import annotations
 import os
 
 import torch
-from torch import nn
 
 import prl_native
+
+from .optim import clip_and_step
 
 
 def wide_info(ppo, D: int):
@@ -234,8 +235,7 @@ class GraphedUpdate:
         if self.fa is not None:
             self.fa.launch(self.ppo._flat_grad)
         else:
-            nn.utils.clip_grad_norm_(self.params, 2.0)
-            self.ppo.optimizer.step()
+            clip_and_step(self.ppo.optimizer, self.params, 2.0)
         return self.loss_out
 
     def _forward_backward(self):
@@ -264,8 +264,7 @@ class GraphedUpdate:
             grads = [p.grad for p in self.params]
             torch._foreach_copy_(grads, [f.view_as(g) for f, g in
                                          zip(self.flat.split(self.sizes), grads)])
-        nn.utils.clip_grad_norm_(self.params, 2.0)
-        self.ppo.optimizer.step()
+        clip_and_step(self.ppo.optimizer, self.params, 2.0)
         self.cursor.add_(1)
 
     def finish(self):

@@ -1,0 +1,669 @@
+// prl_optim.hip — optimizer operators over lists of tensors (include/prl_optim.h): the global
+// gradient norm and one clipped AdamW step with 32-bit or 8-bit moments.
+//
+// The tensors' descriptors travel in the kernels' arguments, a batch of up to 64 tensors per launch:
+// a captured graph then holds them itself, and no table on the device has to outlive a call.  Every
+// tensor is cut into chunks of one workgroup each; a workgroup finds its tensor by comparing its
+// index with the batch's chunk prefix, 64 entries per ballot.
+//
+// One call: list_norm_kernel (per batch; one float64 partial sum per chunk), then list_begin_kernel
+// (one workgroup: folds the partials into the norm and the clip coefficient, advances every
+// tensor's step count and forms its bias corrections in float64), then list_adam32_kernel /
+// list_adam8_kernel per batch.
+#include "prl_common.h"
+#include "../../include/prl_optim.h"
+
+namespace prl {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
+// tensors may start at any element (views of a flat buffer): the types' alignment is one element's,
+// the accesses still are 16 / 8 / 4 bytes wide
+typedef f32x4 f32x4_u __attribute__((aligned(4)));
+typedef u16x4 u16x4_u __attribute__((aligned(2)));
+typedef unsigned u32_u __attribute__((aligned(1)));
+#define PRL_GLOBAL __attribute__((address_space(1)))
+
+constexpr int L_THREADS = 256;
+constexpr int L_BATCH = 64;           // tensors per launch of the norm and the 32-bit step
+constexpr int L_BATCH8 = 48;          // of the 8-bit step (more pointers each; arguments stay under 4 KB)
+constexpr int L_BATCH_BEGIN = 192;    // of list_begin_kernel
+constexpr int L_GROUPS = 16;
+constexpr int L_COEF = 12;            // floats per tensor in the workspace
+constexpr int L_NORM_BLOCKS = 2048;   // partial sums of a norm, besides one per tensor
+
+// per-tensor scalars of a step, formed by list_begin_kernel
+struct Coef {
+  float clip, decay, step_size, inv_bc2_sqrt, omb1, omb2, beta2, eps;
+  unsigned seed, pad[3];
+};
+static_assert(sizeof(Coef) == 4 * L_COEF, "Coef layout");
+
+template <typename T>
+__device__ inline const PRL_GLOBAL T* gptr(const void* p) { return (const PRL_GLOBAL T*)p; }
+template <typename T>
+__device__ inline PRL_GLOBAL T* gptr(void* p) { return (PRL_GLOBAL T*)p; }
+
+// the batch's tensor that workgroup `b` works on: the last one whose first chunk is <= b
+__device__ inline int find_entry(const unsigned* start, int count, unsigned b) {
+  int before = 0;
+  for (int k = 0; k < count; k += 64) {
+    const int i = k + (int)(threadIdx.x & 63);
+    before += __popcll(__ballot(i < count && start[i] <= b));
+  }
+  return __builtin_amdgcn_readfirstlane(before - 1);
+}
+
+// ---- element types ---------------------------------------------------------------------------
+struct F32 {
+  typedef f32x4_u Quad;
+  typedef float One;
+  static __device__ inline f32x4 widen(f32x4 q) { return q; }
+  static __device__ inline f32x4 narrow(f32x4 x) { return x; }
+  static __device__ inline float widen1(float x) { return x; }
+  static __device__ inline float narrow1(float x) { return x; }
+};
+template <typename H>
+struct Half {   // __bf16 / _Float16: conversions round to nearest even
+  typedef u16x4_u Quad;
+  typedef unsigned short One;
+  static __device__ inline float widen1(unsigned short x) { return (float)__builtin_bit_cast(H, x); }
+  static __device__ inline unsigned short narrow1(float x) { return __builtin_bit_cast(unsigned short, (H)x); }
+  static __device__ inline f32x4 widen(u16x4 q) {
+    return f32x4{widen1(q.x), widen1(q.y), widen1(q.z), widen1(q.w)};
+  }
+  static __device__ inline u16x4 narrow(f32x4 x) {
+    return u16x4{narrow1(x.x), narrow1(x.y), narrow1(x.z), narrow1(x.w)};
+  }
+};
+typedef Half<__bf16> BF16;
+typedef Half<_Float16> F16;
+
+// ---- norm ------------------------------------------------------------------------------------
+struct NormArgs {
+  const void* x[L_BATCH];
+  int64_t n[L_BATCH];
+  unsigned start[L_BATCH];
+  unsigned char dtype[L_BATCH];
+  int64_t chunk;
+  int count;
+};
+static_assert(sizeof(NormArgs) <= 4096, "kernel arguments");
+
+template <typename T>
+__device__ inline double norm_chunk(const void* px, int64_t lo, int64_t hi) {
+  const PRL_GLOBAL typename T::One* x = gptr<typename T::One>(px);
+  constexpr int U = 4;
+  double acc = 0.0;
+  int64_t i = lo + 4 * (int64_t)threadIdx.x;
+  for (; i + 4 * L_THREADS * (U - 1) + 4 <= hi; i += 4 * L_THREADS * U) {
+    typename T::Quad q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) q[u] = *(const PRL_GLOBAL typename T::Quad*)(x + i + 4 * L_THREADS * u);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const f32x4 f = T::widen(q[u]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc = fma((double)f[e], (double)f[e], acc);
+    }
+  }
+  for (; i < hi; i += 4 * L_THREADS)
+    for (int e = 0; e < 4; ++e)
+      if (i + e < hi) {
+        const double f = (double)T::widen1(x[i + e]);
+        acc = fma(f, f, acc);
+      }
+  return acc;
+}
+
+__global__ __launch_bounds__(L_THREADS) void list_norm_kernel(const NormArgs a, double* partial) {
+  __shared__ double s_part[L_THREADS / 64];
+  const int e = find_entry(a.start, a.count, blockIdx.x);
+  const int64_t n = a.n[e], lo = (int64_t)(blockIdx.x - a.start[e]) * a.chunk;
+  const int64_t hi = lo + a.chunk < n ? lo + a.chunk : n;
+  double acc;
+  if (a.dtype[e] == PRL_LIST_F32) acc = norm_chunk<F32>(a.x[e], lo, hi);
+  else if (a.dtype[e] == PRL_LIST_BF16) acc = norm_chunk<BF16>(a.x[e], lo, hi);
+  else acc = norm_chunk<F16>(a.x[e], lo, hi);
+  acc = wave_sum_f64_to63(acc);
+  if ((threadIdx.x & 63) == 63) s_part[threadIdx.x >> 6] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double sum = 0.0;
+    for (int w = 0; w < L_THREADS / 64; ++w) sum += s_part[w];
+    partial[blockIdx.x] = sum;
+  }
+}
+
+// ---- once per call: the norm's fold, the step counts, the per-tensor scalars -------------------
+struct BeginArgs {
+  float* step[L_BATCH_BEGIN];
+  unsigned char group[L_BATCH_BEGIN];
+  prl_list_group groups[L_GROUPS];
+  const double* partial;   // n_partial sums to fold into *norm, or n_partial < 0: *norm is ready
+  float* norm;             // or NULL: no clipping
+  Coef* coef;              // of the batch's first tensor
+  int64_t n_partial;
+  float max_norm;
+  int count;
+};
+static_assert(sizeof(BeginArgs) <= 4096, "kernel arguments");
+
+__global__ __launch_bounds__(1024) void list_begin_kernel(const BeginArgs a) {
+  __shared__ double s_part[1024 / 64];
+  __shared__ float s_norm;
+  const int t = threadIdx.x;
+  if (a.norm != nullptr) {
+    if (a.n_partial >= 0) {
+      double acc = 0.0;
+      for (int64_t i = t; i < a.n_partial; i += 1024) acc += a.partial[i];
+      acc = wave_sum_f64_to63(acc);
+      if ((t & 63) == 63) s_part[t >> 6] = acc;
+      __syncthreads();
+      if (t == 0) {
+        double sum = 0.0;
+        for (int w = 0; w < 1024 / 64; ++w) sum += s_part[w];
+        s_norm = (float)sqrt(sum);
+        a.norm[0] = s_norm;
+      }
+    } else if (t == 0) {
+      s_norm = a.norm[0];
+    }
+    __syncthreads();
+  }
+  if (t >= a.count) return;
+  float clip = 1.0f;
+  if (a.norm != nullptr) {
+    clip = a.max_norm / (s_norm + 1e-6f);
+    if (clip > 1.0f) clip = 1.0f;   // a NaN stays
+  }
+  const prl_list_group& g = a.groups[a.group[t]];
+  const double lr = g.lr_dev != nullptr ? (double)g.lr_dev[0] : g.lr;
+  const float step = a.step[t][0] + 1.0f;
+  a.step[t][0] = step;
+  Coef c{};
+  c.clip = clip;
+  c.decay = (float)(1.0 - lr * g.weight_decay);
+  c.step_size = (float)(lr / (1.0 - pow(g.beta1, (double)step)));
+  c.inv_bc2_sqrt = (float)(1.0 / sqrt(1.0 - pow(g.beta2, (double)step)));
+  c.omb1 = (float)(1.0 - g.beta1);
+  c.omb2 = (float)(1.0 - g.beta2);
+  c.beta2 = (float)g.beta2;
+  c.eps = (float)g.eps;
+  c.seed = (unsigned)(int64_t)step * 0x9E3779B1u;
+  a.coef[t] = c;
+}
+
+// ---- the step, 32-bit moments ------------------------------------------------------------------
+struct Adam32Args {
+  void* param[L_BATCH];
+  const void* grad[L_BATCH];
+  float* master[L_BATCH];
+  float* m[L_BATCH];
+  float* v[L_BATCH];
+  int64_t n[L_BATCH];
+  unsigned start[L_BATCH];
+  unsigned which[L_BATCH];   // the tensor's place in the call (its Coef), dtype in the top bits
+  const Coef* coef;
+  int64_t chunk;
+  int count;
+};
+static_assert(sizeof(Adam32Args) <= 4096, "kernel arguments");
+
+__device__ inline float adam_weight(const Coef& c, float w, float m, float rms) {
+  return w * c.decay - c.step_size * (m / (rms * c.inv_bc2_sqrt + c.eps));
+}
+__device__ inline void adam_moments(const Coef& c, float g, float& m, float& v) {
+  g = g * c.clip;
+  m = m + (g - m) * c.omb1;
+  v = v * c.beta2 + (g * g) * c.omb2;
+}
+
+template <typename T, bool MASTER>
+__device__ inline void adam32_chunk(const Coef& c, void* pp, const void* pg, float* pw, float* pm,
+                                    float* pv, int64_t lo, int64_t hi) {
+  PRL_GLOBAL typename T::One* p = gptr<typename T::One>(pp);
+  const PRL_GLOBAL typename T::One* g = gptr<typename T::One>(pg);
+  PRL_GLOBAL float* w = gptr<float>(pw);
+  PRL_GLOBAL float* m = gptr<float>(pm);
+  PRL_GLOBAL float* v = gptr<float>(pv);
+  typedef typename T::Quad Quad;
+  constexpr int U = 2;
+  int64_t i = lo + 4 * (int64_t)threadIdx.x;
+  for (; i + 4 * L_THREADS * (U - 1) + 4 <= hi; i += 4 * L_THREADS * U) {
+    Quad pq[U], gq[U];
+    f32x4 wq[U], mq[U], vq[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t k = i + 4 * L_THREADS * u;
+      if (MASTER) wq[u] = *(const PRL_GLOBAL f32x4_u*)(w + k);
+      else pq[u] = *(const PRL_GLOBAL Quad*)(p + k);
+      gq[u] = *(const PRL_GLOBAL Quad*)(g + k);
+      mq[u] = *(const PRL_GLOBAL f32x4_u*)(m + k);
+      vq[u] = *(const PRL_GLOBAL f32x4_u*)(v + k);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t k = i + 4 * L_THREADS * u;
+      f32x4 x = MASTER ? wq[u] : T::widen(pq[u]);
+      const f32x4 gr = T::widen(gq[u]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float me = mq[u][e], ve = vq[u][e];
+        adam_moments(c, gr[e], me, ve);
+        x[e] = adam_weight(c, x[e], me, sqrtf(ve));
+        mq[u][e] = me;
+        vq[u][e] = ve;
+      }
+      *(PRL_GLOBAL f32x4_u*)(m + k) = mq[u];
+      *(PRL_GLOBAL f32x4_u*)(v + k) = vq[u];
+      if (MASTER) *(PRL_GLOBAL f32x4_u*)(w + k) = x;
+      *(PRL_GLOBAL Quad*)(p + k) = T::narrow(x);
+    }
+  }
+  for (; i < hi; i += 4 * L_THREADS)
+    for (int e = 0; e < 4; ++e)
+      if (i + e < hi) {
+        float me = m[i + e], ve = v[i + e];
+        adam_moments(c, T::widen1(g[i + e]), me, ve);
+        const float x = adam_weight(c, MASTER ? w[i + e] : T::widen1(p[i + e]), me, sqrtf(ve));
+        m[i + e] = me;
+        v[i + e] = ve;
+        if (MASTER) w[i + e] = x;
+        p[i + e] = T::narrow1(x);
+      }
+}
+
+__global__ __launch_bounds__(L_THREADS) void list_adam32_kernel(const Adam32Args a) {
+  const int e = find_entry(a.start, a.count, blockIdx.x);
+  const int64_t n = a.n[e], lo = (int64_t)(blockIdx.x - a.start[e]) * a.chunk;
+  const int64_t hi = lo + a.chunk < n ? lo + a.chunk : n;
+  const unsigned which = a.which[e], dtype = which >> 30;
+  const Coef c = a.coef[which & 0x3fffffffu];
+  void* p = a.param[e];
+  const void* g = a.grad[e];
+  float *w = a.master[e], *m = a.m[e], *v = a.v[e];
+  if (dtype == PRL_LIST_F32) adam32_chunk<F32, false>(c, p, g, w, m, v, lo, hi);
+  else if (dtype == PRL_LIST_BF16) {
+    if (w) adam32_chunk<BF16, true>(c, p, g, w, m, v, lo, hi);
+    else adam32_chunk<BF16, false>(c, p, g, w, m, v, lo, hi);
+  } else {
+    if (w) adam32_chunk<F16, true>(c, p, g, w, m, v, lo, hi);
+    else adam32_chunk<F16, false>(c, p, g, w, m, v, lo, hi);
+  }
+}
+
+// ---- the step, 8-bit moments -------------------------------------------------------------------
+// A block of 256 values is one wave's: 4 consecutive values per lane, so a code quad is one 32-bit
+// word, the block's largest magnitude a wave reduction, and nothing crosses waves.
+struct Adam8Args {
+  void* param[L_BATCH8];
+  const void* grad[L_BATCH8];
+  float* master[L_BATCH8];
+  unsigned* m[L_BATCH8];
+  unsigned* r[L_BATCH8];
+  float* m_scale[L_BATCH8];
+  float* r_scale[L_BATCH8];
+  int64_t n[L_BATCH8];
+  unsigned start[L_BATCH8];
+  unsigned which[L_BATCH8];
+  const Coef* coef;
+  int64_t chunk;
+  int count;
+};
+static_assert(sizeof(Adam8Args) <= 4096, "kernel arguments");
+
+// the largest of an unsigned over the wave, in every lane (as wave_sum_f32_to63, then lane 63's)
+__device__ inline unsigned wave_max_u32(unsigned x) {
+  const auto step = [](unsigned v, int moved) { return v > (unsigned)moved ? v : (unsigned)moved; };
+  x = step(x, __builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, false));
+  x = step(x, __builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, false));
+  x = step(x, __builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xF, 0xF, false));
+  x = step(x, __builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xF, 0xF, false));
+  x = step(x, __builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false));
+  x = step(x, __builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false));
+  return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
+}
+
+// two 16-bit draws for value i of a tensor at this step
+__device__ inline unsigned draw_bits(int64_t i, unsigned seed) {
+  unsigned h = ((unsigned)i + (unsigned)((uint64_t)i >> 32) * 0x85EBCA77u) ^ seed;
+  h = (h ^ (h >> 16)) * 0x7FEB352Du;
+  h = (h ^ (h >> 15)) * 0x846CA68Bu;
+  return h ^ (h >> 16);
+}
+
+// y in [0, 256] to a neighbour on the e4m3 grid: adding 20 random bits below the 3 mantissa bits
+// kept and truncating goes up with probability = the way past the lower neighbour.  Below the
+// smallest normal value the grid is even with the step of the first binade, so y moves there.
+__device__ inline float round_e4m3(float y, unsigned draw16) {
+  const float shift = y < 0x1p-6f ? 0x1p-6f : 0.0f;
+  const unsigned u = (__float_as_uint(y + shift) + (draw16 << 4)) & 0xFFF00000u;
+  return __uint_as_float(u) - shift;
+}
+
+struct Scale {
+  float k, store;   // 256 / A (0: the block is held as zeros), and A as stored
+};
+__device__ inline Scale block_scale(unsigned max_bits) {
+  const float A = __uint_as_float(max_bits);
+  Scale s;
+  s.k = 0.0f;
+  s.store = 0.0f;
+  if (max_bits >= 0x7f800000u) s.store = __uint_as_float(0x7fc00000u);
+  else if (A >= 0x1p-118f) {
+    s.k = 256.0f / A;
+    s.store = A;
+  }
+  return s;
+}
+
+template <typename T, bool MASTER>
+__device__ inline void adam8_block(const Coef& c, void* pp, const void* pg, float* pw, unsigned* pm,
+                                   unsigned* pr, float* pms, float* prs, int64_t base, int64_t n) {
+  typedef typename T::Quad Quad;
+  const int64_t i = base + 4 * (int64_t)(threadIdx.x & 63), b = base / PRL_LIST_BLOCK;
+  PRL_GLOBAL typename T::One* p = gptr<typename T::One>(pp) + i;
+  const PRL_GLOBAL typename T::One* g = gptr<typename T::One>(pg) + i;
+  PRL_GLOBAL float* w = gptr<float>(pw) + (MASTER ? i : 0);
+  PRL_GLOBAL unsigned char* mc = gptr<unsigned char>((void*)pm) + i;
+  PRL_GLOBAL unsigned char* rc = gptr<unsigned char>((void*)pr) + i;
+  const bool whole = i + 4 <= n;
+  const int left = whole ? 4 : (i < n ? (int)(n - i) : 0);
+  f32x4 x = {0.f, 0.f, 0.f, 0.f}, gr = x;
+  unsigned mq = 0, rq = 0;
+  if (whole) {
+    gr = T::widen(*(const PRL_GLOBAL Quad*)g);
+    x = MASTER ? *(const PRL_GLOBAL f32x4_u*)w : T::widen(*(const PRL_GLOBAL Quad*)p);
+    mq = *(const PRL_GLOBAL u32_u*)mc;
+    rq = *(const PRL_GLOBAL u32_u*)rc;
+  } else {
+    for (int e = 0; e < 3; ++e)
+      if (e < left) {
+        gr[e] = T::widen1(g[e]);
+        x[e] = MASTER ? w[e] : T::widen1(p[e]);
+        mq |= (unsigned)mc[e] << (8 * e);
+        rq |= (unsigned)rc[e] << (8 * e);
+      }
+  }
+  const float ms = gptr<float>(pms)[b] * 0x1p-8f, rs = gptr<float>(prs)[b] * 0x1p-8f;
+  float m[4] = {__builtin_amdgcn_cvt_f32_fp8(mq, 0), __builtin_amdgcn_cvt_f32_fp8(mq, 1),
+                __builtin_amdgcn_cvt_f32_fp8(mq, 2), __builtin_amdgcn_cvt_f32_fp8(mq, 3)};
+  float r[4] = {__builtin_amdgcn_cvt_f32_fp8(rq, 0), __builtin_amdgcn_cvt_f32_fp8(rq, 1),
+                __builtin_amdgcn_cvt_f32_fp8(rq, 2), __builtin_amdgcn_cvt_f32_fp8(rq, 3)};
+  unsigned m_max = 0, r_max = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    m[e] = m[e] * ms;
+    r[e] = r[e] * rs;
+    float v = r[e] * r[e];
+    adam_moments(c, gr[e], m[e], v);
+    r[e] = sqrtf(v);
+    if (e >= left) m[e] = r[e] = 0.0f;   // past the tensor's end (a NaN scale or clip must not count twice)
+    const unsigned mb = __float_as_uint(m[e]) & 0x7fffffffu, rb = __float_as_uint(r[e]) & 0x7fffffffu;
+    m_max = m_max > mb ? m_max : mb;
+    r_max = r_max > rb ? r_max : rb;
+  }
+  const Scale sm = block_scale(wave_max_u32(m_max)), sr = block_scale(wave_max_u32(r_max));
+  float mo[4], ro[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[e] = adam_weight(c, x[e], m[e], r[e]);
+    const unsigned d = draw_bits(i + e, c.seed);
+    // k == 0: zeros (a product with a NaN or an infinity would not be)
+    const float ym = sm.k > 0.0f ? fminf(fabsf(m[e]) * sm.k, 256.0f) : 0.0f;
+    const float yr = sr.k > 0.0f ? fminf(r[e] * sr.k, 256.0f) : 0.0f;
+    mo[e] = copysignf(round_e4m3(ym, d & 0xffffu), m[e]);
+    ro[e] = round_e4m3(yr, d >> 16);
+    if (r[e] > 0.0f && sr.k > 0.0f) ro[e] = fmaxf(ro[e], 0x1p-9f);
+  }
+  int mw = __builtin_amdgcn_cvt_pk_fp8_f32(mo[0], mo[1], 0, false);
+  mw = __builtin_amdgcn_cvt_pk_fp8_f32(mo[2], mo[3], mw, true);
+  int rw = __builtin_amdgcn_cvt_pk_fp8_f32(ro[0], ro[1], 0, false);
+  rw = __builtin_amdgcn_cvt_pk_fp8_f32(ro[2], ro[3], rw, true);
+  if (whole) {
+    if (MASTER) *(PRL_GLOBAL f32x4_u*)w = x;
+    *(PRL_GLOBAL Quad*)p = T::narrow(x);
+    *(PRL_GLOBAL u32_u*)mc = (unsigned)mw;
+    *(PRL_GLOBAL u32_u*)rc = (unsigned)rw;
+  } else {
+    for (int e = 0; e < 3; ++e)
+      if (e < left) {
+        if (MASTER) w[e] = x[e];
+        p[e] = T::narrow1(x[e]);
+        mc[e] = (unsigned char)((unsigned)mw >> (8 * e));
+        rc[e] = (unsigned char)((unsigned)rw >> (8 * e));
+      }
+  }
+  if ((threadIdx.x & 63) == 0) {
+    gptr<float>(pms)[b] = sm.store;
+    gptr<float>(prs)[b] = sr.store;
+  }
+}
+
+template <typename T, bool MASTER>
+__device__ inline void adam8_chunk(const Coef& c, const Adam8Args& a, int e, int64_t lo, int64_t hi, int64_t n) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (int64_t base = lo + wave * PRL_LIST_BLOCK; base < hi; base += L_THREADS / 64 * PRL_LIST_BLOCK)
+    adam8_block<T, MASTER>(c, a.param[e], a.grad[e], a.master[e], a.m[e], a.r[e], a.m_scale[e], a.r_scale[e], base, n);
+}
+
+__global__ __launch_bounds__(L_THREADS) void list_adam8_kernel(const Adam8Args a) {
+  const int e = find_entry(a.start, a.count, blockIdx.x);
+  const int64_t n = a.n[e], lo = (int64_t)(blockIdx.x - a.start[e]) * a.chunk;
+  const int64_t hi = lo + a.chunk < n ? lo + a.chunk : n;
+  const unsigned which = a.which[e], dtype = which >> 30;
+  const Coef c = a.coef[which & 0x3fffffffu];
+  const bool master = a.master[e] != nullptr;
+  if (dtype == PRL_LIST_F32) adam8_chunk<F32, false>(c, a, e, lo, hi, n);
+  else if (dtype == PRL_LIST_BF16) {
+    if (master) adam8_chunk<BF16, true>(c, a, e, lo, hi, n);
+    else adam8_chunk<BF16, false>(c, a, e, lo, hi, n);
+  } else {
+    if (master) adam8_chunk<F16, true>(c, a, e, lo, hi, n);
+    else adam8_chunk<F16, false>(c, a, e, lo, hi, n);
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------
+inline int64_t list_total(const prl_list_entry* e, int64_t count) {
+  int64_t total = 0;
+  for (int64_t i = 0; i < count; ++i) total += e[i].numel;
+  return total;
+}
+
+// the partial sums of all grads' squares into partial[0 .. *n_partial)
+int launch_norm(const prl_list_entry* e, int64_t count, double* partial, int64_t* n_partial, hipStream_t st) {
+  const int64_t tile = 4 * L_THREADS * 4;
+  NormArgs a{};
+  a.chunk = tile * (1 + list_total(e, count) / (tile * L_NORM_BLOCKS));
+  int64_t done = 0, blocks = 0;
+  for (int64_t i = 0; i <= count; ++i) {
+    if (a.count == L_BATCH || (i == count && a.count > 0)) {
+      hipLaunchKernelGGL(list_norm_kernel, dim3((unsigned)blocks), dim3(L_THREADS), 0, st, a, partial + done);
+      PRL_LAUNCH_CHECK("list_norm");
+      done += blocks;
+      blocks = 0;
+      a.count = 0;
+    }
+    if (i == count || e[i].numel == 0) continue;
+    a.x[a.count] = e[i].grad;
+    a.n[a.count] = e[i].numel;
+    a.start[a.count] = (unsigned)blocks;
+    a.dtype[a.count] = (unsigned char)e[i].dtype;
+    ++a.count;
+    blocks += cdiv(e[i].numel, a.chunk);
+  }
+  *n_partial = done;
+  return PRL_OK;
+}
+
+// list_begin_kernel over all tensors: batches of at most L_BATCH_BEGIN tensors and L_GROUPS groups
+int launch_begin(const prl_list_entry* e, int64_t count, const prl_list_group* groups, float max_norm,
+                 float* norm, const double* partial, int64_t n_partial, Coef* coef, hipStream_t st) {
+  BeginArgs a{};
+  a.partial = partial;
+  a.norm = norm;
+  a.n_partial = n_partial;
+  a.max_norm = max_norm;
+  int64_t first = 0, of[L_GROUPS];
+  int n_of = 0;
+  for (int64_t i = 0;; ++i) {
+    int g = 0;
+    if (i < count) {
+      while (g < n_of && of[g] != e[i].group) ++g;
+    }
+    if (i == count || a.count == L_BATCH_BEGIN || g == L_GROUPS) {
+      a.coef = coef + first;
+      hipLaunchKernelGGL(list_begin_kernel, dim3(1), dim3(1024), 0, st, a);
+      PRL_LAUNCH_CHECK("list_begin");
+      a.n_partial = -1;   // later batches read the norm that the first one folded
+      first = i;
+      a.count = n_of = g = 0;
+      if (i == count) return PRL_OK;
+    }
+    if (g == n_of) {
+      of[n_of] = e[i].group;
+      a.groups[n_of++] = groups[e[i].group];
+    }
+    a.step[a.count] = e[i].step;
+    a.group[a.count] = (unsigned char)g;
+    ++a.count;
+  }
+}
+
+int launch_adam32(const prl_list_entry* e, int64_t count, const Coef* coef, hipStream_t st) {
+  Adam32Args a{};
+  a.coef = coef;
+  a.chunk = 4 * L_THREADS * 4;
+  int64_t blocks = 0;
+  for (int64_t i = 0; i <= count; ++i) {
+    if (a.count == L_BATCH || (i == count && a.count > 0)) {
+      hipLaunchKernelGGL(list_adam32_kernel, dim3((unsigned)blocks), dim3(L_THREADS), 0, st, a);
+      PRL_LAUNCH_CHECK("list_adam32");
+      blocks = 0;
+      a.count = 0;
+    }
+    if (i == count || e[i].numel == 0 || e[i].bits != 32) continue;
+    const int k = a.count++;
+    a.param[k] = e[i].param;
+    a.grad[k] = e[i].grad;
+    a.master[k] = e[i].master;
+    a.m[k] = static_cast<float*>(e[i].exp_avg);
+    a.v[k] = static_cast<float*>(e[i].second);
+    a.n[k] = e[i].numel;
+    a.start[k] = (unsigned)blocks;
+    a.which[k] = (unsigned)i | (unsigned)e[i].dtype << 30;
+    blocks += cdiv(e[i].numel, a.chunk);
+  }
+  return PRL_OK;
+}
+
+int launch_adam8(const prl_list_entry* e, int64_t count, const Coef* coef, hipStream_t st) {
+  Adam8Args a{};
+  a.coef = coef;
+  a.chunk = 4 * L_THREADS * 4;
+  int64_t blocks = 0;
+  for (int64_t i = 0; i <= count; ++i) {
+    if (a.count == L_BATCH8 || (i == count && a.count > 0)) {
+      hipLaunchKernelGGL(list_adam8_kernel, dim3((unsigned)blocks), dim3(L_THREADS), 0, st, a);
+      PRL_LAUNCH_CHECK("list_adam8");
+      blocks = 0;
+      a.count = 0;
+    }
+    if (i == count || e[i].numel == 0 || e[i].bits != 8) continue;
+    const int k = a.count++;
+    a.param[k] = e[i].param;
+    a.grad[k] = e[i].grad;
+    a.master[k] = e[i].master;
+    a.m[k] = static_cast<unsigned*>(e[i].exp_avg);
+    a.r[k] = static_cast<unsigned*>(e[i].second);
+    a.m_scale[k] = e[i].exp_avg_scale;
+    a.r_scale[k] = e[i].second_scale;
+    a.n[k] = e[i].numel;
+    a.start[k] = (unsigned)blocks;
+    a.which[k] = (unsigned)i | (unsigned)e[i].dtype << 30;
+    blocks += cdiv(e[i].numel, a.chunk);
+  }
+  return PRL_OK;
+}
+
+// sizes and types; a list's total stays below 2^40 values, so every launch's grid fits
+int check_list(const char* what, const prl_list_entry* e, int64_t count) {
+  PRL_REQUIRE(count >= 0 && count < (1 << 24), "%s: %lld tensors", what, (long long)count);
+  PRL_REQUIRE(count == 0 || e != nullptr, "%s: null entries", what);
+  int64_t total = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    PRL_REQUIRE(e[i].numel >= 0 && e[i].numel < (int64_t)1 << 40, "%s: tensor %lld: bad size %lld", what,
+                (long long)i, (long long)e[i].numel);
+    total += e[i].numel;
+    PRL_REQUIRE(total < (int64_t)1 << 40, "%s: list too large", what);
+    PRL_REQUIRE(e[i].dtype >= PRL_LIST_F32 && e[i].dtype <= PRL_LIST_F16, "%s: tensor %lld: unknown type %d", what,
+                (long long)i, (int)e[i].dtype);
+    PRL_REQUIRE(e[i].numel == 0 || e[i].grad, "%s: tensor %lld: null grad", what, (long long)i);
+    PRL_REQUIRE((reinterpret_cast<uintptr_t>(e[i].grad) & (e[i].dtype == PRL_LIST_F32 ? 3u : 1u)) == 0,
+                "%s: tensor %lld: grad not aligned to its type", what, (long long)i);
+  }
+  return PRL_OK;
+}
+
+}  // namespace prl
+
+using namespace prl;
+
+extern "C" int64_t prl_list_workspace_bytes(int64_t count) {
+  if (count < 0) return -1;
+  return (int64_t)sizeof(Coef) * count + 8 * (L_NORM_BLOCKS + count);
+}
+
+extern "C" int prl_list_norm(const prl_list_entry* entries, int64_t count, float* norm, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  if (int rc = check_list("prl_list_norm", entries, count)) return rc;
+  PRL_REQUIRE(norm && workspace, "prl_list_norm: null pointer");
+  PRL_REQUIRE(aligned16(workspace) && workspace_bytes >= prl_list_workspace_bytes(count),
+              "prl_list_norm: workspace too small or not 16-B aligned");
+  Coef* coef = static_cast<Coef*>(workspace);
+  double* partial = reinterpret_cast<double*>(coef + count);
+  int64_t n_partial = 0;
+  if (int rc = launch_norm(entries, count, partial, &n_partial, as_stream(stream))) return rc;
+  return launch_begin(entries, 0, nullptr, 0.0f, norm, partial, n_partial, coef, as_stream(stream));
+}
+
+extern "C" int prl_list_adamw(const prl_list_entry* entries, int64_t count, const prl_list_group* groups,
+                              int64_t n_groups, float max_norm, float* norm, void* workspace,
+                              int64_t workspace_bytes, void* stream) {
+  if (int rc = check_list("prl_list_adamw", entries, count)) return rc;
+  if (count == 0 && norm == nullptr) return PRL_OK;
+  PRL_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= prl_list_workspace_bytes(count),
+              "prl_list_adamw: workspace null, too small or not 16-B aligned");
+  PRL_REQUIRE(norm == nullptr || max_norm >= 0.0f, "prl_list_adamw: max_norm %g", (double)max_norm);
+  PRL_REQUIRE(count == 0 || groups, "prl_list_adamw: null groups");
+  for (int64_t i = 0; i < count; ++i) {
+    const prl_list_entry& e = entries[i];
+    PRL_REQUIRE(e.bits == 32 || e.bits == 8, "prl_list_adamw: tensor %lld: moments in %d bits", (long long)i, (int)e.bits);
+    PRL_REQUIRE(e.group >= 0 && e.group < n_groups, "prl_list_adamw: tensor %lld: group %lld of %lld", (long long)i,
+                (long long)e.group, (long long)n_groups);
+    PRL_REQUIRE(e.step, "prl_list_adamw: tensor %lld: null step", (long long)i);
+    PRL_REQUIRE(e.master == nullptr || e.dtype != PRL_LIST_F32, "prl_list_adamw: tensor %lld: a float32 param has no master",
+                (long long)i);
+    if (e.numel == 0) continue;
+    PRL_REQUIRE(e.param && e.exp_avg && e.second && (e.bits == 32 || (e.exp_avg_scale && e.second_scale)),
+                "prl_list_adamw: tensor %lld: null pointer", (long long)i);
+    const uintptr_t p = reinterpret_cast<uintptr_t>(e.param);
+    const uintptr_t s = reinterpret_cast<uintptr_t>(e.exp_avg) | reinterpret_cast<uintptr_t>(e.second);
+    const uintptr_t f = reinterpret_cast<uintptr_t>(e.master) | reinterpret_cast<uintptr_t>(e.exp_avg_scale) |
+                        reinterpret_cast<uintptr_t>(e.second_scale) | reinterpret_cast<uintptr_t>(e.step);
+    PRL_REQUIRE((p & (e.dtype == PRL_LIST_F32 ? 3u : 1u)) == 0 && (e.bits == 8 || (s & 3u) == 0) && (f & 3u) == 0,
+                "prl_list_adamw: tensor %lld: a pointer not aligned to its type", (long long)i);
+  }
+  hipStream_t st = as_stream(stream);
+  Coef* coef = static_cast<Coef*>(workspace);
+  double* partial = reinterpret_cast<double*>(coef + count);
+  int64_t n_partial = 0;
+  if (norm) {
+    if (int rc = launch_norm(entries, count, partial, &n_partial, st)) return rc;
+  }
+  if (int rc = launch_begin(entries, count, groups, max_norm, norm, partial, n_partial, coef, st)) return rc;
+  if (int rc = launch_adam32(entries, count, coef, st)) return rc;
+  return launch_adam8(entries, count, coef, st);
+}

@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import os
 import threading
+from array import array
 
 import torch
 
@@ -114,6 +115,12 @@ SIGNATURES = {
     "prl_ppo_grad_fold_step": [_P] * 7 + [_I64, _F32, _I32, _I32, _I32] + [_P] * 5
                               + [_I64, _I32, _I64, _F32] + _UPD_SCALARS + [_P, _P, _P, _I64, _P],
 }
+# include/prl_optim.h: the optimizer operators over lists of tensors
+OPTIM_SIGNATURES = {
+    "prl_list_workspace_bytes": [_I64],
+    "prl_list_norm": [_P, _I64, _P, _P, _I64, _P],
+    "prl_list_adamw": [_P, _I64, _P, _I64, _F32, _P, _P, _I64, _P],
+}
 _RESTYPES = {"prl_last_error": ctypes.c_char_p, "prl_source_id": ctypes.c_char_p,
              "prl_ppo_update_last_plan": None, "prl_workspace_bytes": _I64,
              "prl_rnd_pred_grad_ws_floats": _I64, "prl_dp_xbuf_bytes": _I64,
@@ -121,7 +128,8 @@ _RESTYPES = {"prl_last_error": ctypes.c_char_p, "prl_source_id": ctypes.c_char_p
              "prl_ppo_update_set_repl": _I32, "prl_ppo_update_set_split": _I32,
              "prl_ppo_update_wb_check": _I32,
              "prl_ppo_update_dp_split": _I32,
-             "prl_ppo_image_floats": _I64, "prl_colsum_partial_floats": _I64}
+             "prl_ppo_image_floats": _I64, "prl_colsum_partial_floats": _I64,
+             "prl_list_workspace_bytes": _I64}
 
 _lib = None
 _lock = threading.Lock()
@@ -156,7 +164,7 @@ def lib():
                     raise RuntimeError(f"libprl_hip.so not found at {LIB_PATH}: build it with "
                                        "parallel-reinforcement-learning_amd/csrc/build.py")
                 L = ctypes.CDLL(LIB_PATH)
-                for name, args in SIGNATURES.items():
+                for name, args in (*SIGNATURES.items(), *OPTIM_SIGNATURES.items()):
                     try:
                         fn = getattr(L, name)
                     except AttributeError:
@@ -792,6 +800,62 @@ def flat_adamw(params, exp_avg, exp_avg_sq, step, grad, lr, beta1, beta2, eps, w
         float(weight_decay), float(max_norm), _dev(total_norm, torch.float32, "total_norm"),
         _stream()), "prl_flat_adamw")
     return total_norm[:1]
+
+
+LIST_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+LIST_BLOCK = 256          # values per scale of an 8-bit moment (include/prl_optim.h)
+LIST_ENTRY_WORDS = 11     # int64 words of a prl_list_entry
+LIST_GROUP_WORDS = 6      # 8-byte words of a prl_list_group
+
+
+def list_entry(param=0, grad=0, master=0, exp_avg=0, second=0, exp_avg_scale=0, second_scale=0,
+               step=0, numel=0, dtype=0, bits=32, group=0) -> tuple:
+    """One prl_list_entry as its int64 words (device addresses, 0 = NULL)."""
+    return (param, grad, master, exp_avg, second, exp_avg_scale, second_scale, step, numel,
+            dtype | bits << 32, group)
+
+
+def _list_call(device, call):
+    """call(stream) with `device` current and its current stream (a list's tensors may live on
+    another device than the current one)."""
+    if device.index == torch.cuda.current_device():
+        return call(torch.cuda.current_stream().cuda_stream)
+    with torch.cuda.device(device):
+        return call(torch.cuda.current_stream().cuda_stream)
+
+
+def list_norm(entries: array, device: torch.device) -> torch.Tensor:
+    """prl_list_norm over the entries' grads (an array("q") of prl_list_entry words): a new 0-dim
+    f32 tensor.  Scratch is allocated per call, so a captured graph owns its own."""
+    count = len(entries) // LIST_ENTRY_WORDS
+    need = int(lib().prl_list_workspace_bytes(count))
+
+    def call(stream):
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        _check(lib().prl_list_norm(entries.buffer_info()[0], count, norm.data_ptr(), ws.data_ptr(),
+                                   need, stream), "prl_list_norm")
+        return norm
+    return _list_call(device, call)
+
+
+def list_adamw(entries: array, groups: array, device: torch.device, max_norm=None):
+    """prl_list_adamw: one AdamW step of every entry (array("q") of prl_list_entry words; groups:
+    array("d") / bytes of prl_list_group words).  With max_norm the gradients are clipped by their
+    global norm, which is returned (a new 0-dim f32 tensor); None otherwise."""
+    count = len(entries) // LIST_ENTRY_WORDS
+    need = int(lib().prl_list_workspace_bytes(count))
+
+    def call(stream):
+        norm = None if max_norm is None else torch.empty((), dtype=torch.float32, device=device)
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        _check(lib().prl_list_adamw(entries.buffer_info()[0], count, groups.buffer_info()[0],
+                                    len(groups) // LIST_GROUP_WORDS,
+                                    0.0 if max_norm is None else max_norm,
+                                    None if norm is None else norm.data_ptr(), ws.data_ptr(), need,
+                                    stream), "prl_list_adamw")
+        return norm
+    return _list_call(device, call)
 
 
 def ppo_update_last_plan() -> dict:

@@ -1,0 +1,135 @@
+"""The list optimizer without a GPU: its C-ABI (include/prl_optim.h) and that header's symbols, what
+it refuses before anything is launched, and the float64 restatement the GPU tests rely on."""
+import ctypes
+import os
+import re
+from array import array
+
+import pytest
+import torch
+
+import optim_ref as R
+from conftest import ROOT
+
+
+def test_header_symbols_are_exported_and_bound():
+    import prl_native
+    hdr = open(os.path.join(ROOT, "include", "prl_optim.h")).read()
+    syms = sorted(set(re.findall(r"^\s*(?:int|int64_t)\s+(prl_list_\w+)\s*\(", hdr, re.M)))
+    assert syms == sorted(prl_native.OPTIM_SIGNATURES)
+    assert all(hasattr(prl_native.lib(), s) for s in syms)
+    assert len(prl_native.list_entry()) == prl_native.LIST_ENTRY_WORDS
+    assert int(re.search(r"#define PRL_LIST_BLOCK (\d+)", hdr).group(1)) == prl_native.LIST_BLOCK
+
+
+def _adamw(entries, groups=((1e-3, 0.9, 0.999, 1e-8, 0.0, 0),), n_groups=None, ws=1 << 20, norm=None, max_norm=1.0, bytes_=None):
+    """prl_list_adamw's status on a list that it must refuse (addresses are never touched)."""
+    import struct
+    import prl_native
+    L = prl_native.lib()
+    table = array("q", [w for e in entries for w in e])
+    g = b"".join(struct.pack("5dq", *x) for x in groups)
+    rc = L.prl_list_adamw(table.buffer_info()[0] if entries else None, len(entries), g, len(groups) if n_groups is None else n_groups,
+                          max_norm, norm, ws, L.prl_list_workspace_bytes(len(entries)) if bytes_ is None else bytes_, None)
+    return rc, L.prl_last_error().decode()
+
+
+def test_c_entry_refuses_bad_lists():
+    from prl_native import list_entry
+    ok = dict(param=4096, grad=8192, exp_avg=12288, second=16384, step=20480, numel=10)
+    cases = [
+        (dict(ok, dtype=3), "unknown type"), (dict(ok, dtype=-1), "unknown type"),
+        (dict(ok, numel=-1), "bad size"), (dict(ok, numel=1 << 40), "bad size"),
+        (dict(ok, bits=16), "moments in 16 bits"), (dict(ok, group=1), "group 1 of 1"), (dict(ok, group=-1), "group -1"),
+        (dict(ok, step=0), "null step"), (dict(ok, grad=0), "null grad"), (dict(ok, param=0), "null pointer"),
+        (dict(ok, second=0), "null pointer"), (dict(ok, bits=8), "null pointer"),
+        (dict(ok, master=4096), "has no master"), (dict(ok, grad=8194), "grad not aligned"),
+        (dict(ok, param=4098), "not aligned"), (dict(ok, exp_avg=12289), "not aligned"), (dict(ok, step=20481), "not aligned"),
+    ]
+    for e, text in cases:
+        rc, msg = _adamw([list_entry(**ok), list_entry(**e)])
+        assert rc == -1 and text in msg, (e, msg)
+    assert _adamw([list_entry(**ok)], bytes_=64)[0] == -1
+    assert _adamw([list_entry(**ok)], ws=None)[0] == -1
+    assert _adamw([list_entry(**ok)], ws=(1 << 20) + 8)[0] == -1
+    assert _adamw([list_entry(**ok)], norm=4096, max_norm=-1.0)[0] == -1
+    assert _adamw([list_entry(**ok)], norm=4096, max_norm=float("nan"))[0] == -1
+    assert _adamw([])[0] == 0          # nothing to do, nothing launched
+    import prl_native
+    L = prl_native.lib()
+    assert L.prl_list_workspace_bytes(-1) == -1
+    assert L.prl_list_norm(None, 1, 4096, 4096, 1 << 20, None) == -1
+    assert L.prl_list_norm(None, -1, 4096, 4096, 1 << 20, None) == -1
+    assert L.prl_list_norm(None, 0, None, 4096, 1 << 20, None) == -1
+    total = array("q", [w for _ in range(3) for w in list_entry(grad=4096, numel=(1 << 40) - 1)])
+    assert L.prl_list_norm(total.buffer_info()[0], 3, 4096, 4096, 1 << 20, None) == -1
+    assert "too large" in L.prl_last_error().decode()
+
+
+def test_python_refusals():
+    from PPO.optim import AdamW, grad_norm
+    p = torch.nn.Parameter(torch.ones(6))
+    for kw in (dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)), dict(lr=-1.0), dict(eps=-1.0), dict(weight_decay=-1.0),
+               dict(state_bits=16)):
+        with pytest.raises(ValueError):
+            AdamW([p], **kw)
+    with pytest.raises(ValueError, match="share memory"):
+        AdamW([p, torch.nn.Parameter(p.detach()[2:4])])
+    opt = AdamW([p])
+    with pytest.raises(ValueError, match="share memory"):
+        opt.add_param_group(dict(params=[torch.nn.Parameter(p.detach()[:1])]))
+    assert len(opt.param_groups) == 1
+    p.grad = torch.ones(6)
+    with pytest.raises(ValueError, match="device tensor"):
+        opt.step()
+    with pytest.raises(ValueError, match="device tensor"):
+        grad_norm([p.grad])
+    assert torch.equal(p.detach(), torch.ones(6)) and not opt.state[p].get("exp_avg", None)
+
+
+def test_learn_keeps_its_step_for_other_optimizers():
+    """clip_and_step is clip_grad_norm_ + step() for any optimizer that is not this AdamW."""
+    from PPO.optim import clip_and_step
+    p = torch.nn.Parameter(torch.ones(4))
+    q = torch.nn.Parameter(torch.ones(4))
+    p.grad, q.grad = torch.full((4,), 3.0), torch.full((4,), 3.0)
+    clip_and_step(torch.optim.SGD([p], lr=0.1), [p], 2.0)
+    torch.nn.utils.clip_grad_norm_([q], 2.0)
+    torch.optim.SGD([q], lr=0.1).step()
+    assert torch.equal(p, q) and torch.equal(p.grad, q.grad)
+
+
+# ---------------------------------------------------------------------------------- the restatement itself
+def test_restatement_is_torch_adamw():
+    gen = torch.Generator().manual_seed(0)
+    w = torch.randn(50, generator=gen, dtype=torch.float64)
+    p = torch.nn.Parameter(w.clone())
+    opt = torch.optim.AdamW([p], lr=1e-2, betas=(0.8, 0.95), eps=1e-6, weight_decay=0.1)
+    m = v = torch.zeros(50, dtype=torch.float64)
+    for t in (1, 2, 3):
+        g = torch.randn(50, generator=gen, dtype=torch.float64)
+        p.grad = g.clone()
+        norm = float(torch.nn.utils.clip_grad_norm_([p], 0.5))
+        opt.step()
+        assert abs(R.norm64([g]) - norm) < 1e-12 * norm
+        w, m, v, *_ = R.step64(w, g, m, v, t, 1e-2, (0.8, 0.95), 1e-6, 0.1, R.clip64(norm, 0.5))
+        assert torch.allclose(w, p.detach(), rtol=1e-12, atol=1e-14)
+
+
+def test_restatement_rounds_to_neighbours_on_the_e4m3_grid():
+    gen = torch.Generator().manual_seed(0)
+    x = torch.randn(1000, generator=gen, dtype=torch.float64) * 10.0 ** torch.linspace(-8, 0, 1000, dtype=torch.float64)
+    d, _ = R.draws(1000, 5)
+    assert int(d.min()) >= 0 and int(d.max()) < 65536 and abs(float(d.double().mean()) / 32768 - 1) < 0.1
+    A, q, low, high = R.quantise(x, d, 0.0)
+    assert torch.equal(q.float().to(torch.float8_e4m3fn).double(), q)             # on the grid
+    y = x / A.repeat_interleave(256)[:1000] * 256
+    unit = torch.exp2(torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -6))) - 3)
+    assert bool(((q - y).abs() < unit).all())
+    lowest = R.quantise(x, d * 0, 2.0 ** -9)[1]
+    assert bool((lowest.abs() >= 2.0 ** -9).all())                                  # nothing becomes 0
+    # two values may be held where, and only where, the error reaches over a border
+    assert float((low < high).double().mean()) < 0.01
+    _, q, low, high = R.quantise(x, d, 0.0, x.abs() * 1e-3)
+    assert bool(((low <= q.abs()) & (q.abs() <= high)).all())
+    assert 0.001 < float((low < high).double().mean()) < 0.1

@@ -1,0 +1,545 @@
+"""The optimizer operators over lists of tensors (csrc/prl_optim.hip, PPO/optim.py) against their
+float64 restatement (optim_ref.py).  Tolerances: float32 evaluations are held to the roundings that
+optim_ref.step64 counts, per value; a 16-bit parameter to half a step of its type more; 8-bit codes are
+equal to the restatement's unless the value before rounding lies within its own float32 error of a
+border, and then one that a value within that error rounds to."""
+import math
+
+import pytest
+import torch
+
+import optim_ref as R
+
+pytestmark = pytest.mark.gpu
+SIZES = [1, 3, 4, 5, 255, 256, 257, 1023, 4096, 4097, 20001, 0, 17411]
+
+
+def _optim():
+    import PPO.optim
+    return PPO.optim
+
+
+def _make(sizes, dtype, seed, packed=True, lead=1):
+    """Parameters and gradients as views of flat buffers (`lead` values before the first: odd
+    offsets)."""
+    gen = torch.Generator().manual_seed(seed)
+    out, grads = [], []
+    if packed:
+        flat = torch.zeros(lead + sum(sizes), dtype=dtype, device="cuda")
+        gflat = torch.zeros_like(flat)
+    at = lead
+    for n in sizes:
+        w = (torch.randn(n, generator=gen) * 0.05 + 0.01).to(dtype).cuda()
+        g = (torch.randn(n, generator=gen) * 10.0 ** (torch.rand(1, generator=gen) * 3 - 3)).to(dtype).cuda()
+        if packed:
+            flat[at:at + n], gflat[at:at + n] = w, g
+            w, g = flat[at:at + n], gflat[at:at + n]
+            at += n
+        p = torch.nn.Parameter(w)
+        p.grad = g
+        out.append(p)
+        grads.append(g)
+    return out, grads
+
+
+def _moments(st, bits, n):
+    """The moments of a state in float64 on the CPU: (m, rms squared)."""
+    if bits == 32:
+        return st["exp_avg"].reshape(-1).cpu().double(), st["exp_avg_sq"].reshape(-1).cpu().double()
+
+    def read(k):
+        q = st[k].reshape(-1).cpu().double()
+        return q * st[k + "_scale"].cpu().double().repeat_interleave(256)[:n] / 256
+    return read("exp_avg"), read("exp_rms").square()
+
+
+def _check_step(opt, params, before, c, t, hyper, bits):
+    """Every parameter and state against one float64 step from `before`."""
+    for p, (w, g, m, v) in zip(params, before):
+        n = p.numel()
+        w1, m1, v1, ew, em, ev = R.step64(w, g, m, v, t, *hyper, c)
+        st = opt.state[p]
+        assert float(st["step"]) == t
+        got = st["master"] if "master" in st else p.detach()
+        extra = 0.0 if got.dtype == torch.float32 else R.HALF_STEP[p.dtype] * (w1.abs() + ew) + 2.0 ** -25
+        err = (got.reshape(-1).cpu().double() - w1).abs()
+        assert bool((err <= ew + extra).all()), (n, float((err - ew - extra).max()))
+        if "master" in st:   # the parameter is its master's rounding
+            assert torch.equal(p.detach(), st["master"].to(p.dtype))
+        if bits == 32:
+            gm, gv = _moments(st, 32, n)
+            assert bool(((gm - m1).abs() <= em).all()) and bool(((gv - v1).abs() <= ev).all()), n
+            continue
+        dm, dr = R.draws(n, t)
+        r1 = v1.sqrt()
+        er = torch.where(r1 > 0, ev / (2 * r1.clamp(min=1e-70)), torch.zeros_like(r1)) + 2 * R.U32 * r1
+        for k, x, d, least, e in (("exp_avg", m1, dm, 0.0, em), ("exp_rms", r1, dr, 2.0 ** -9, er)):
+            A, q, low, high = R.quantise(x, d, least, e)
+            ga, gq = st[k + "_scale"].cpu().double(), st[k].reshape(-1).cpu().double()
+            ea = torch.nn.functional.pad(e, (0, -n % 256)).view(-1, 256).amax(1)
+            assert bool(((ga - A).abs() <= ea).all()), (n, k)
+            off = gq != q
+            assert bool(((gq.abs() >= low) & (gq.abs() <= high) & (gq * x >= 0)).all()), (n, k, int(off.sum()))
+            # few lie so near a border, except where v is below float32's normal values: its steps
+            # there are 2^-149 whatever v is, all of it may be lost (v < 2^-150 is 0 in float32)
+            assert int(off.sum()) <= 0.02 * n + int((v1 < 2.0 ** -126).sum()), (n, k)
+
+
+def _before(opt, params, bits, fresh):
+    out = []
+    for p in params:
+        n, st = p.numel(), opt.state.get(p)
+        w = (st["master"] if st and "master" in st else p.detach()).reshape(-1).cpu().double()
+        m, v = (torch.zeros(n, dtype=torch.float64),) * 2 if fresh else _moments(st, bits, n)
+        out.append((w, p.grad.reshape(-1).cpu().double(), m, v))
+    return out
+
+
+# ---------------------------------------------------------------------------------- norm
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_grad_norm(dtype):
+    """sqrt of the float64 sum of squares: off by one float32 rounding."""
+    for sizes in ([1], [3], SIZES, [7] * 300, [200_003]):
+        _, grads = _make(sizes, dtype, len(sizes))
+        got, want = float(_optim().grad_norm(grads)), R.norm64(grads)
+        assert abs(got - want) <= 1.01 * R.U32 * want, sizes
+
+
+def test_grad_norm_edges():
+    f = _optim().grad_norm
+    x = torch.randn(64, 48, device="cuda")
+    assert abs(float(f([x.t()])) - R.norm64([x])) <= 1.01 * R.U32 * R.norm64([x])    # strided
+    assert float(f(x.new_empty(0))) == 0.0 and float(f([x.new_empty(0), x.new_zeros(5)])) == 0.0
+    big = torch.full((1000,), 1e30, device="cuda")         # squares past float32
+    assert abs(float(f([big])) / (1e30 * math.sqrt(1000)) - 1) < 1e-6
+    mixed = [x, x.bfloat16(), x.half()]
+    assert abs(float(f(mixed)) - R.norm64(mixed)) <= 1.01 * R.U32 * R.norm64(mixed)
+    assert math.isnan(float(f([x, x.new_full((3,), float("nan"))])))
+    assert math.isinf(float(f([x.new_full((3,), float("inf")), x])))
+    a = f([x])
+    b = f([x])
+    assert torch.equal(a, b) and a.shape == ()
+
+
+# ---------------------------------------------------------------------------------- the step
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype,master", [(torch.float32, False), (torch.bfloat16, False),
+                                          (torch.bfloat16, True), (torch.float16, False),
+                                          (torch.float16, True)])
+@pytest.mark.parametrize("max_norm", [None, 0.5])
+def test_adamw_steps(bits, dtype, master, max_norm):
+    """Three steps (the first from empty state) over odd sizes at odd offsets."""
+    params, grads = _make(SIZES, dtype, 11)
+    hyper = (1e-2, (0.9, 0.999), 1e-8, 0.1)
+    opt = _optim().AdamW(params, lr=hyper[0], betas=hyper[1], eps=hyper[2], weight_decay=hyper[3],
+                         state_bits=bits, master=master)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for t in (1, 2, 3):
+        before = _before(opt, params, bits, t == 1)
+        norm = R.norm64(grads)
+        kept = [g.clone() for g in grads]
+        opt.step(max_norm=max_norm)
+        if max_norm is None:
+            assert opt.total_norm is None
+        else:
+            assert norm > max_norm and abs(float(opt.total_norm) - norm) <= 1.01 * R.U32 * norm
+        assert all(torch.equal(a, b) for a, b in zip(kept, grads))     # gradients stay as they are
+        _check_step(opt, params, before, R.clip64(norm, max_norm), t, hyper, bits)
+        for g in grads:
+            g.copy_(torch.randn(g.shape, generator=gen, device="cuda") * 0.03)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_many_tensors_groups_and_types(bits):
+    """More tensors than a launch holds, more groups than list_begin's batch, types mixed, separate
+    allocations, one group's lr on the device, some parameters without a gradient."""
+    groups, every = [], []
+    for i in range(19):
+        dtype = (torch.float32, torch.bfloat16, torch.float16)[i % 3]
+        params, _ = _make([1 + (37 * i + 11 * j) % 700 for j in range(13)], dtype, i, packed=i % 2 == 0)
+        lr = 1e-3 * (i + 1)
+        groups.append(dict(params=params, lr=torch.full((), lr, device="cuda") if i == 4 else lr,
+                           betas=(0.8 + 0.01 * i, 0.99), weight_decay=0.01 * i, master=i % 2 == 1))
+        every.append((params, (float(torch.tensor(lr)) if i == 4 else lr, (0.8 + 0.01 * i, 0.99), 1e-8, 0.01 * i)))
+    without = every[3][0][2]
+    without.grad = None
+    old = without.detach().clone()
+    opt = _optim().AdamW(groups, state_bits=bits)
+    grads = [p.grad for params, _ in every for p in params if p.grad is not None]
+    norm = R.norm64(grads)
+    befores = [_before(opt, [p for p in params if p.grad is not None], bits, True) for params, _ in every]
+    opt.step(max_norm=1.0)
+    assert torch.equal(without.detach(), old) and not opt.state.get(without)
+    for (params, hyper), before in zip(every, befores):
+        _check_step(opt, [p for p in params if p.grad is not None], before, R.clip64(norm, 1.0), 1, hyper, bits)
+
+
+def test_adamw_matches_torch_and_exchanges_state():
+    """float32, 32-bit moments: four clipped steps beside torch's clip_grad_norm_ + AdamW, the state
+    moved from one to the other in between by state_dict().  Both are float32 evaluations of the same
+    step: per step each is off by at most ~6 U of a weight and 16 U of an update of <= 10 lr here."""
+    params, grads = _make(SIZES, torch.float32, 5)
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    a = _optim().AdamW(params, lr=1e-3)
+    b = torch.optim.AdamW(twins, lr=1e-3)
+    for t in range(4):
+        for g, q in zip(grads, twins):
+            g.copy_(torch.randn_like(g) * 0.1)
+            q.grad = g.clone()
+        a.step(max_norm=2.0)
+        norm = torch.nn.utils.clip_grad_norm_(twins, 2.0)
+        b.step()
+        assert abs(float(a.total_norm) - float(norm)) <= 1e-6 * float(norm)
+        for p, q in zip(params, twins):
+            if p.numel():
+                top = float(q.detach().abs().max())
+                assert float((p - q).detach().abs().max()) <= (t + 1) * 2 * R.U32 * (6 * top + 16 * 1e-2)
+        if t == 1:     # swap the states
+            sa, sb = a.state_dict(), b.state_dict()
+            a = _optim().AdamW(params, lr=1e-3)
+            b = torch.optim.AdamW(twins, lr=1e-3)
+            a.load_state_dict(sb)
+            b.load_state_dict(sa)
+    for p in params:
+        assert float(a.state[p]["step"]) == 4.0
+
+
+@pytest.mark.parametrize("dtype,master", [(torch.float32, False), (torch.bfloat16, True)])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_dict_round_trip(bits, dtype, master):
+    """A saved and loaded optimizer goes on with the same bits; the state keeps its types."""
+    params, grads = _make(SIZES, dtype, 6)
+    a = _optim().AdamW(params, state_bits=bits, master=master)
+    a.step()
+    saved = a.state_dict()
+    kept = [p.detach().clone() for p in params]
+    types = {k: v.dtype for k, v in a.state[params[4]].items()}
+    a.step()
+    want = [p.detach().clone() for p in params]
+    with torch.no_grad():
+        for p, k in zip(params, kept):
+            p.copy_(k)
+    b = _optim().AdamW(params, state_bits=bits, master=master)
+    # `saved` holds a's own tensors, which its second step moved: rebuild the first step's state
+    c = _optim().AdamW([torch.nn.Parameter(p.detach().clone()) for p in params], state_bits=bits, master=master)
+    del saved, c
+    fresh, fgrads = _make(SIZES, dtype, 6)
+    d = _optim().AdamW(fresh, state_bits=bits, master=master)
+    d.step()
+    import copy
+    b.load_state_dict(copy.deepcopy(d.state_dict()))
+    assert {k: v.dtype for k, v in b.state[params[4]].items()} == types
+    b.step()
+    assert all(torch.equal(p.detach(), w) for p, w in zip(params, want))
+
+
+# ---------------------------------------------------------------------------------- values that are not finite
+def test_adamw_nonfinite_gradients():
+    """32-bit: as torch (a NaN stays at its value).  8-bit: its block of 256 turns NaN, no other."""
+    for bad in (float("nan"), float("inf")):
+        p = torch.nn.Parameter(torch.ones(1000, device="cuda"))
+        p.grad = torch.full((1000,), 0.1, device="cuda")
+        p.grad[300] = bad
+        opt = _optim().AdamW([p])
+        opt.step()
+        assert torch.isfinite(p).sum() == 999 and math.isnan(p.detach()[300])
+        q = torch.nn.Parameter(torch.ones(1000, device="cuda"))
+        q.grad = p.grad.clone()
+        opt = _optim().AdamW([q], state_bits=8)
+        opt.step()
+        assert torch.isfinite(q).sum() == 999 and math.isnan(q.detach()[300])
+        scale = opt.state[q]["exp_avg_scale"]
+        assert math.isnan(float(scale[1])) and torch.isfinite(scale).sum() == 3
+        q.grad[300] = 0.1
+        opt.step()
+        nan = torch.isnan(q).cpu()
+        assert bool(nan[256:512].all()) and not bool(nan[:256].any()) and not bool(nan[512:].any())
+    # the norm of a list with a NaN: every parameter NaN, as clip_grad_norm_ + step; an infinite norm: c = 0
+    p = torch.nn.Parameter(torch.ones(8, device="cuda"))
+    p.grad = torch.tensor([1.0] * 7 + [float("nan")], device="cuda")
+    _optim().AdamW([p]).step(max_norm=1.0)
+    assert bool(torch.isnan(p).all())
+    p = torch.nn.Parameter(torch.ones(8, device="cuda"))
+    p.grad = torch.tensor([1.0] * 7 + [float("inf")], device="cuda")
+    opt = _optim().AdamW([p], weight_decay=0.0)
+    opt.step(max_norm=1.0)
+    assert p[:7].tolist() == [1.0] * 7 and math.isnan(p.detach()[7]) and math.isinf(float(opt.total_norm))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_zero_tiny_and_huge_values(bits):
+    """All-zero gradients and max_norm = 0 (no update but the decay, moments zero), blocks of tiny
+    and huge values."""
+    for scale, max_norm in ((0.0, None), (1.0, 0.0), (1e-30, None), (1e-18, None), (1e15, None)):
+        p = torch.nn.Parameter(torch.linspace(-1, 1, 700, device="cuda"))
+        p.grad = torch.linspace(-1, 1, 700, device="cuda") * scale
+        opt = _optim().AdamW([p], lr=1e-2, eps=1e-8, state_bits=bits)
+        before = _before(opt, [p], bits, True)
+        opt.step(max_norm=max_norm)
+        assert bool(torch.isfinite(p).all())
+        c = R.clip64(R.norm64([p.grad]), max_norm)
+        _check_step(opt, [p], before, c, 1, (1e-2, (0.9, 0.999), 1e-8, 1e-2), bits)
+    # 8-bit: below 2^-118 a block is held as zeros
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    p.grad = torch.full((300,), 1e-36, device="cuda")
+    opt = _optim().AdamW([p], state_bits=8)
+    opt.step()
+    assert opt.state[p]["exp_avg"].float().abs().max() == 0 and opt.state[p]["exp_avg_scale"].abs().max() == 0
+
+
+def test_adamw8_rounding_is_unbiased():
+    """The mean of what is held over many values equals the mean of what was to be held: 2^20 equal
+    gradients (but one larger in each block, which fixes the scale) whose quotient lies a third of
+    the way between two codes.  The share s of upper codes has a standard deviation of at most
+    1 / (2 * 2^10): five of them are 0.0025; 16-bit draws shift it by at most 2^-16."""
+    n = 1 << 20
+    lower, unit = 40.0, 4.0                       # e4m3 neighbours 40 and 44
+    target = (lower + unit / 3) / 256.0           # of the block's largest
+    g = torch.full((n,), target, device="cuda")
+    g[::256] = 1.0
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
+    p.grad = g
+    opt = _optim().AdamW([p], state_bits=8)
+    opt.step()
+    st = opt.state[p]
+    for k in ("exp_avg", "exp_rms"):
+        q = st[k].float().view(-1, 256)
+        assert bool((q[:, 0] == 256).all())
+        q = q[:, 1:]
+        assert bool(((q == lower) | (q == lower + unit)).all())
+        assert abs(float((q > lower).double().mean()) - 1 / 3) <= 0.0025 + 2.0 ** -16, k
+    # the draws of exp_avg and exp_rms, and of two steps, are not the same ones
+    up = (st["exp_avg"].float() > lower) != (st["exp_rms"].float() > lower)
+    assert float(up.double().mean()) > 0.3
+
+
+def test_adamw8_second_moment_follows_smaller_gradients():
+    """After a spike in half of the values, their second moment decays with beta2 towards the rest's,
+    in codes whose steps are 6 to 12 %, far above one step's change of 0.05 %: with rounding to the
+    nearest it would stay where it is.  Expected after T steps: r^2 = 0.001 * 100 * 0.999^T + (1 -
+    0.999^T) (in units of the rest); the noise of the rounding over 2^16 values averages out below
+    2 %, and E[r] against sqrt(E[r^2]) differs by the spread of r, at most 25 %."""
+    n, T = 1 << 16, 1500
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
+    opt = _optim().AdamW([p], lr=0.0, state_bits=8, weight_decay=0.0)
+    g = torch.ones(n, device="cuda")
+    spike = g.clone()
+    spike[::2] = 10.0
+    p.grad = spike
+    for _ in range(30):
+        opt.step()
+    p.grad = g
+    for _ in range(T):
+        opt.step()
+    st = opt.state[p]
+    r = st["exp_rms"].float() * st["exp_rms_scale"].repeat_interleave(256) / 256
+    keep = 0.999 ** T
+    high = math.sqrt((1 - 0.999 ** 30) * 100 * keep + 1 - keep)
+    low = math.sqrt((1 - 0.999 ** 30) * keep + 1 - keep)
+    assert abs(float(r[::2].mean()) / high - 1) < 0.25 and abs(float(r[1::2].mean()) / low - 1) < 0.25
+
+
+# ---------------------------------------------------------------------------------- streams, graphs, layouts
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_captured_step_replays_as_eager(bits):
+    """A captured step (norm, clip, update, counts, a device lr that changes between replays) replayed
+    with eager work and synchronizations in between: the bits of eager steps.  Two graphs of two
+    optimizers replay beside each other on two streams."""
+    sets = []
+    for k in range(2):
+        params, grads = _make([5, 300, 4096, 777], torch.bfloat16, 20 + k)
+        twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+        for p, q in zip(params, twins):
+            q.grad = p.grad
+        lr = torch.full((), 1e-2, device="cuda")
+        a = _optim().AdamW(params, lr=lr, state_bits=bits, master=k == 1)
+        b = _optim().AdamW(twins, lr=lr, state_bits=bits, master=k == 1)
+        a.step(max_norm=0.5)
+        b.step(max_norm=0.5)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            a.step(max_norm=0.5)
+        sets.append((params, grads, twins, lr, a, b, graph, a.total_norm, torch.cuda.Stream()))
+    for r in range(4):
+        for params, grads, twins, lr, a, b, graph, norm, s in sets:
+            lr.fill_(1e-2 / (r + 1))
+            for g in grads:
+                g.copy_(torch.randn(g.shape, device="cuda") * 0.1)
+        torch.cuda.synchronize()
+        for x in sets:
+            with torch.cuda.stream(x[8]):
+                x[6].replay()
+        torch.cuda.synchronize()
+        for params, grads, twins, lr, a, b, graph, norm, s in sets:
+            b.step(max_norm=0.5)
+            torch.cuda.synchronize()
+            assert torch.equal(norm, b.total_norm)
+            for p, q in zip(params, twins):
+                assert torch.equal(p, q)
+                sa, sb = a.state[p], b.state[q]
+                assert all(torch.equal(sa[k].view(torch.uint8) if sa[k].dtype.itemsize == 1 else sa[k],
+                                       sb[k].view(torch.uint8) if sb[k].dtype.itemsize == 1 else sb[k]) for k in sa)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_is_deterministic_and_follows_replaced_tensors(bits):
+    """The same steps give the same bits, on another stream too; gradients that are strided, and
+    parameters and gradients that move to other memory between steps, are followed."""
+    runs = []
+    for way in range(2):
+        params, grads = _make([64 * 48, 1000], torch.float32, 8)
+        params[0].data = params[0].data.view(64, 48)
+        params[0].grad = grads[0].view(64, 48)
+        opt = _optim().AdamW(params, state_bits=bits)
+        s = torch.cuda.Stream() if way else torch.cuda.current_stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            opt.step(max_norm=1.0)
+            if way:     # the same gradient with other strides, the parameter elsewhere
+                params[0].grad = params[0].grad.t().contiguous().t()
+                assert not params[0].grad.is_contiguous()
+                params[1].data = params[1].data.clone()
+                params[1].grad = params[1].grad.clone()
+            opt.step(max_norm=1.0)
+        torch.cuda.synchronize()
+        runs.append([p.detach().clone() for p in params] + [opt.state[p]["exp_avg"].float() for p in params])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_adamw_past_32_bits():
+    """A tensor of 2^32 + 515 values: offsets, block numbers and the draws' high word past 32 bits."""
+    n = (1 << 32) + 515
+    p = torch.nn.Parameter(torch.empty(n, dtype=torch.bfloat16, device="cuda").fill_(0.5))
+    p.grad = torch.empty(n, dtype=torch.bfloat16, device="cuda").fill_(2.0 ** -9)
+    tail = slice(n - 515 - 1024, n)
+    gen = torch.Generator().manual_seed(1)
+    p.grad[tail] = (torch.randn(515 + 1024, generator=gen) * 0.01).bfloat16().cuda()
+    opt = _optim().AdamW([p], lr=1e-2, state_bits=8)
+    opt.step(max_norm=1e9)
+    g = p.grad[tail].cpu().double()
+    norm = math.sqrt((n - 1539) * 2.0 ** -18 + float(g.square().sum()))
+    assert abs(float(opt.total_norm) - norm) <= 1.01 * R.U32 * norm
+    zero = torch.zeros(1539, dtype=torch.float64)
+    w1, m1, v1, ew, em, ev = R.step64(zero + 0.5, g, zero, zero, 1, 1e-2, (0.9, 0.999), 1e-8, 1e-2, 1.0)
+    err = (p.detach()[tail].cpu().double() - w1).abs()
+    assert bool((err <= ew + R.HALF_STEP[torch.bfloat16] * (w1.abs() + ew)).all())
+    dm, _ = R.draws(1539, 1, first=n - 1539)
+    A, q, low, high = R.quantise(m1, dm, 0.0, em)       # n - 1539 is a multiple of 256: blocks as the tensor's
+    assert (n - 1539) % 256 == 0
+    st = opt.state[p]
+    got = st["exp_avg"][tail].cpu().double()
+    off = got != q
+    assert bool(((got.abs() >= low) & (got.abs() <= high)).all()) and float(off.double().mean()) < 0.02
+    assert bool(((st["exp_avg_scale"][-7:].cpu().double() - A).abs() <= 16 * R.U32 * A).all())
+
+
+# ---------------------------------------------------------------------------------- together, as learn() uses them
+def _learn(make_optimizer, use_graphs, use_fused=False, cont=False, mb=256):
+    from PPO import PPO
+    torch.manual_seed(0)
+    D, A = (3, 1) if cont else (4, 2)
+    ppo = PPO(cont, D, A, action_scaling=2.0 if cont else None, lr=1e-3, k_epochs=3, batch_size=64, mini_batch_size=mb)
+    ppo.show_progress = False
+    ppo.use_fused, ppo.use_graphs = use_fused, use_graphs
+    if make_optimizer is not None:
+        ppo.optimizer = make_optimizer(ppo.policy.parameters())
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    n = 2000 + 37
+    S = torch.randn(n, D, generator=gen, device="cuda")
+    act = (torch.randn(n, A, generator=gen, device="cuda") if cont
+           else torch.randint(0, A, (n,), generator=gen, device="cuda").float())
+    ppo.memory.push_device(S, act, torch.randn(n, generator=gen, device="cuda"),
+                           (torch.rand(n, generator=gen, device="cuda") < 0.01).float())
+    ppo.learn()
+    torch.cuda.synchronize()
+    return ppo
+
+
+def test_learn_steps_through_the_list_adamw():
+    """PPO.learn() with this AdamW: the update engine takes it with 32-bit moments and leaves it the
+    state; with 8-bit moments the per-step paths run (the native gradient step, and autograd captured and
+    eager with the same bits), and end near the 32-bit run (24 steps of at most ~lr each could part
+    the weights by 2 * 24 * lr)."""
+    AdamW = _optim().AdamW
+    engine = _learn(lambda p: AdamW(p, lr=1e-3), True, use_fused=True)
+    plain = _learn(None, True, use_fused=True)
+    assert engine.last_update_path == plain.last_update_path == "fused"
+    for p, q in zip(engine.policy.parameters(), plain.policy.parameters()):
+        assert torch.equal(p, q)
+        assert torch.equal(engine.optimizer.state[p]["exp_avg"], plain.optimizer.state[q]["exp_avg"])
+    assert float(engine.optimizer.state[p]["step"]) == 24.0
+    native = _learn(lambda p: AdamW(p, lr=1e-3, state_bits=8), True, use_fused=True)
+    assert native.last_update_path == "graph" and native._last_graphed.wide is not None
+    graph = _learn(lambda p: AdamW(p, lr=1e-3, state_bits=8), True)
+    eager = _learn(lambda p: AdamW(p, lr=1e-3, state_bits=8), False)
+    assert graph.last_update_path == "graph" and graph.last_graph_replays > 0 and eager.last_update_path == "eager"
+    for p, q, r, x in zip(*(o.policy.parameters() for o in (graph, eager, plain, native))):
+        assert torch.equal(p, q) and bool(torch.isfinite(p).all()) and bool(torch.isfinite(x).all())
+        assert float((p - r).detach().abs().max()) <= 2 * 24 * 1e-3
+        assert float((x - r).detach().abs().max()) <= 2 * 24 * 1e-3
+        for o, w in ((graph, p), (native, x)):
+            st = o.optimizer.state[w]
+            assert st["exp_avg"].dtype == torch.float8_e4m3fn and float(st["step"]) == 24.0
+
+
+def test_learn_wide_policy_and_rnd_with_8_bit_moments():
+    """The wide step (348 observations, 17 actions) and the RND predictor's update with 8-bit moments."""
+    from PPO import PPO
+    torch.manual_seed(0)
+    ppo = PPO(True, 348, 17, action_scaling=1.0, k_epochs=2, batch_size=64, mini_batch_size=512, use_RND=True)
+    ppo.show_progress = False
+    AdamW = _optim().AdamW
+    ppo.optimizer = AdamW(ppo.policy.parameters(), state_bits=8)
+    ppo.rnd.optimizer = AdamW(ppo.rnd.pred_net.parameters(), lr=1e-3, state_bits=8)
+    old = [p.detach().clone() for p in list(ppo.policy.parameters()) + list(ppo.rnd.pred_net.parameters())]
+    n = 1100
+    ppo.memory.push_device(torch.randn(n, 348, device="cuda"), torch.randn(n, 17, device="cuda") * 0.1,
+                           torch.randn(n, device="cuda"), (torch.rand(n, device="cuda") < 0.01).float())
+    ppo.learn()
+    torch.cuda.synchronize()
+    for o, steps in ((ppo.optimizer, 6.0), (ppo.rnd.optimizer, 3.0)):
+        for g in o.param_groups:
+            assert all(float(o.state[p]["step"]) == steps for p in g["params"])
+    new = list(ppo.policy.parameters()) + list(ppo.rnd.pred_net.parameters())
+    assert all(bool(torch.isfinite(p).all()) and not torch.equal(p, o) for p, o in zip(new, old))
+
+
+def test_refusals_on_the_device():
+    O = _optim()
+    p = torch.nn.Parameter(torch.ones(10, device="cuda"))
+    with pytest.raises(ValueError, match="share memory"):
+        O.AdamW([p, torch.nn.Parameter(p.detach()[3:5])])
+    with pytest.raises(ValueError, match="contiguous"):
+        O.AdamW([torch.nn.Parameter(torch.ones(4, 6, device="cuda").t())])
+    with pytest.raises(ValueError, match="float32, bfloat16 or float16"):
+        O.AdamW([torch.nn.Parameter(torch.ones(4, dtype=torch.float64, device="cuda"))])
+    with pytest.raises(ValueError, match="device tensor"):
+        O.grad_norm([p, torch.ones(3)])
+    with pytest.raises(ValueError, match="at least one"):
+        O.grad_norm([])
+    opt = O.AdamW([p], state_bits=8)
+    p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError, match="max_norm"):
+        opt.step(max_norm=-1.0)
+    with pytest.raises(ValueError, match="max_norm"):
+        opt.step(max_norm=float("nan"))
+    opt.step()
+    opt.state[p]["exp_rms"] = opt.state[p]["exp_rms"].float()
+    with pytest.raises(ValueError, match="exp_rms"):
+        opt.step()
+    del opt.state[p]["exp_rms"]
+    with pytest.raises(ValueError, match="no exp_rms"):
+        opt.step()
+    q = torch.nn.Parameter(torch.ones(10, device="cuda"))
+    two = O.AdamW([p, q])
+    q.grad = torch.ones_like(q)
+    two.step()
+    two.state[q]["step"] = two.state[p]["step"]
+    with pytest.raises(ValueError, match="step count"):
+        two.step()
+    fresh = O.AdamW([q])
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="outside it first"):
+        with torch.cuda.graph(graph):
+            fresh.step()
