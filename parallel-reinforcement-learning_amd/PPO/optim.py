@@ -14,16 +14,35 @@ from __future__ import annotations
 
 import struct
 from array import array
+from itertools import chain, repeat
+from operator import attrgetter, is_
 
 import torch
 from torch import nn
 
 import prl_native
 
-_entry = prl_native.list_entry
-_BLOCK = prl_native.LIST_BLOCK
+_BLOCK, _WORDS, _DTYPES = prl_native.LIST_BLOCK, prl_native.LIST_ENTRY_WORDS, prl_native.LIST_DTYPES
 # state keys of the two forms of the moments: (first, second, first's scales, second's scales)
 _MOMENTS = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_rms", "exp_avg_scale", "exp_rms_scale")}
+# one attribute of every tensor of a list by map(): some 40 ns a tensor, a loop's body costs several times that
+_ptr, _numel, _contiguous, _device = (torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous,
+                                      torch.Tensor.get_device)
+_dtype, _layout = attrgetter("dtype"), attrgetter("layout")
+
+
+def _dense(tensors, device, name):
+    """The tensors, contiguous (those that are not: copies), after checking that they are dense
+    device tensors of a known type on one device."""
+    if not all(map(is_, map(_layout, tensors), repeat(torch.strided))) or any(d != device for d in map(_device, tensors)):
+        for t in tensors:
+            if t.layout is not torch.strided or not t.is_cuda:
+                raise ValueError(f"{name} must be a dense device tensor (got {t.layout} on {t.device})")
+        raise ValueError(f"{name}: all must be on one device (got {sorted({str(t.device) for t in tensors})})")
+    for t in tensors:
+        if t.dtype not in _DTYPES:
+            raise ValueError(f"{name} must be float32, bfloat16 or float16 (got {t.dtype})")
+    return tensors if all(map(_contiguous, tensors)) else [t.detach().contiguous() for t in tensors]
 
 
 def grad_norm(tensors) -> torch.Tensor:
@@ -33,23 +52,12 @@ def grad_norm(tensors) -> torch.Tensor:
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not tensors:
         raise ValueError("grad_norm needs at least one tensor")
-    device, table, keep = tensors[0].device, array("q"), []
-    for i, t in enumerate(tensors):
-        _check_tensor(t, device, f"tensor {i}")
-        if not t.is_contiguous():
-            t = t.contiguous()
-            keep.append(t)
-        table.extend(_entry(grad=t.data_ptr(), numel=t.numel(), dtype=prl_native.LIST_DTYPES[t.dtype]))
-    return prl_native.list_norm(table, device)
-
-
-def _check_tensor(t, device, name):
-    if t.is_sparse or not t.is_cuda:
-        raise ValueError(f"{name} must be a dense device tensor (got {t.layout} on {t.device})")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the others on {device}")
-    if t.dtype not in prl_native.LIST_DTYPES:
-        raise ValueError(f"{name} must be float32, bfloat16 or float16 (got {t.dtype})")
+    tensors = _dense(tensors, max(tensors[0].get_device(), 0), "a tensor of the list")
+    table = array("q", bytes(8 * _WORDS * len(tensors)))
+    table[1::_WORDS] = array("q", map(_ptr, tensors))
+    table[8::_WORDS] = array("q", map(_numel, tensors))
+    table[9::_WORDS] = array("q", map(_DTYPES.__getitem__, map(_dtype, tensors)))
+    return prl_native.list_norm(table, tensors[0].device)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -77,8 +85,7 @@ class AdamW(torch.optim.Optimizer):
                  state_bits: int = 32, master: bool = False):
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
                         state_bits=state_bits, master=master, capturable=True)
-        self._checked = {}      # parameter -> the state tensors found right the last time
-        self._last_rows = self._last_table = None
+        self._plan = None       # the last step's list, laid out (_Plan)
         self.total_norm = None
         super().__init__(params, defaults)
 
@@ -129,12 +136,12 @@ class AdamW(torch.optim.Optimizer):
             st["master"] = p.detach().float()
 
     def _check_state(self, p, group, st):
-        """The state tensors of p, in the order of the entry's pointers."""
+        """p's state tensors by the entry's columns (2 .. 7); None: a null pointer."""
         bits, numel = group["state_bits"], p.numel()
         half_master = group["master"] and p.dtype != torch.float32
-        names = _MOMENTS[bits] + ("step",) + (("master",) if half_master else ())
-        found = []
-        for k in names:
+        columns = [None] * 6
+        for k, column in zip(_MOMENTS[bits] + ("step",) + (("master",) if half_master else ()),
+                             ((1, 2) if bits == 32 else (1, 2, 3, 4)) + (5, 0)):
             t = st.get(k)
             if not torch.is_tensor(t):
                 raise ValueError(f"the state of a parameter has no {k} (state_bits={bits}, master={group['master']})")
@@ -143,9 +150,8 @@ class AdamW(torch.optim.Optimizer):
             if t.dtype != want or t.numel() != size or t.device != p.device or not t.is_contiguous():
                 raise ValueError(f"{k} must be {size} contiguous {want} values on {p.device} "
                                  f"(got {t.numel()} {t.dtype} on {t.device})")
-            found.append(t)
-        self._checked[p] = (bits, numel, tuple(names), found)
-        return self._checked[p]
+            columns[column] = t
+        return columns
 
     def load_state_dict(self, state_dict):
         """torch's, except that the state keeps its own types (torch casts every state tensor to the
@@ -162,8 +168,7 @@ class AdamW(torch.optim.Optimizer):
                     v = torch.as_tensor(v, dtype=torch.float32).reshape(())
                 if torch.is_tensor(v):
                     self.state[p][k] = v.detach().to(device=p.device, copy=True)
-        self._checked.clear()
-        self._last_rows = None
+        self._plan = None
 
     def flat_state(self) -> bool:
         """Whether this optimizer's step is one AdamW step of float32 parameters with float32 moments
@@ -175,13 +180,9 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._checked, self._last_rows, self._last_table = {}, None, None
-
-    def __getstate__(self):
-        return {**super().__getstate__(), "total_norm": self.total_norm}
+        self._plan, self.total_norm = None, None
 
     # ------------------------------------------------------------------ step
-    @torch.no_grad()
     def step(self, closure=None, *, max_norm=None):
         """One step of every parameter that has a gradient; with max_norm (>= 0) the gradients of
         all groups are clipped together by their global norm first (p.grad stays as it is)."""
@@ -191,46 +192,20 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         if max_norm is not None and not max_norm >= 0.0:
             raise ValueError(f"max_norm must not be negative (got {max_norm})")
-        rows, groups, keep, device = [], bytearray(), [], None
-        dtypes, state, checked = prl_native.LIST_DTYPES, self.state, self._checked
-        for index, group in enumerate(self.param_groups):
-            groups += self._group_words(group)
-            for p in group["params"]:
-                g = p.grad
-                if g is None:
-                    continue
-                if device is None:
-                    device = p.device
-                if p.device != device or g.dtype != p.dtype or not p.is_contiguous() or not p.is_cuda:
-                    _check_tensor(p, device, "a parameter")
-                    raise ValueError("a parameter must be contiguous and its gradient of its type")
-                if not g.is_contiguous() or g.is_sparse:
-                    _check_tensor(g, device, "a gradient")
-                    g = g.contiguous()
-                    keep.append(g)
-                st = state[p]
-                if not st:
-                    self._init_state(p, group, st)
-                known = checked.get(p)
-                if (known is None or known[0] != group["state_bits"] or known[1] != p.numel()
-                        or any(st.get(k) is not t for k, t in zip(known[2], known[3]))):
-                    known = self._check_state(p, group, st)
-                bits, numel, names, t = known
-                rows.extend(_entry(p.data_ptr(), g.data_ptr(),
-                                   t[-1].data_ptr() if names[-1] == "master" else 0,
-                                   t[0].data_ptr(), t[1].data_ptr(),
-                                   t[2].data_ptr() if bits == 8 else 0,
-                                   t[3].data_ptr() if bits == 8 else 0,
-                                   t[4 if bits == 8 else 2].data_ptr(), numel, dtypes[p.dtype], bits, index))
-        if not rows:
-            self.total_norm = None if max_norm is None else torch.zeros((), device=self.param_groups[0]["params"][0].device)
-            return loss
-        if rows != self._last_rows:     # the arguments' table; the tensors' values are never kept
-            steps = rows[7::prl_native.LIST_ENTRY_WORDS]
-            if len(set(steps)) < len(steps):
-                raise ValueError("two parameters share a step count tensor: each needs its own")
-            self._last_rows, self._last_table = rows, array("q", rows)
-        self.total_norm = prl_native.list_adamw(self._last_table, array("q", bytes(groups)), device,
+        groups = self.param_groups
+        params = [p for group in groups for p in group["params"]]
+        grads = [p.grad for p in params]
+        plan = self._plan
+        if plan is None or not plan.holds(groups, params, grads, self.state):
+            plan = self._plan = None     # (dropped first: laying out may refuse)
+            plan = _Plan(self, groups, params, grads)
+            if not plan.params:
+                self.total_norm = None if max_norm is None else torch.zeros((), device=params[0].device)
+                return loss
+            self._plan = plan
+        words = b"".join(map(self._group_words, groups))
+        table, keep = plan.fill(grads)
+        self.total_norm = prl_native.list_adamw(table, array("q", words), plan.device,
                                                 None if max_norm is None else float(max_norm))
         return loss
 
@@ -245,6 +220,83 @@ class AdamW(torch.optim.Optimizer):
             else:
                 lr = float(lr)
         return struct.pack("5dq", lr, beta1, beta2, group["eps"], group["weight_decay"], on_device)
+
+
+class _Plan:
+    """A step's list as prl_list_entry words, and what to compare before it serves the next step:
+    which parameters step, with which state tensors, and where those lie.  Gradients are looked up
+    anew by every step; a list of which anything else differs is laid out, and checked, again."""
+
+    def __init__(self, opt, groups, params, grads):
+        self.every, self.without = params, list(map(is_, grads, repeat(None)))
+        self.settings = self._settings(groups)
+        index = [(i, g) for i, g in enumerate(groups) for _ in g["params"]]
+        chosen = [(p, g, *ig) for p, g, ig in zip(params, grads, index) if g is not None]
+        self.params = [c[0] for c in chosen]
+        if not chosen:
+            return
+        self.device = self.params[0].device
+        _dense(self.params, max(self.params[0].get_device(), 0), "a parameter")
+        columns = []
+        for p, g, _, group in chosen:
+            if not p.is_contiguous():
+                raise ValueError("a parameter must be contiguous")
+            if g.dtype != p.dtype or g.numel() != p.numel():
+                raise ValueError(f"a gradient must be of its parameter's type and size (got {g.numel()} {g.dtype} "
+                                 f"for {p.numel()} {p.dtype})")
+            st = opt.state[p]
+            if not st:
+                opt._init_state(p, group, st)
+            columns.append(opt._check_state(p, group, st))
+        if len(set(map(_ptr, (c[5] for c in columns)))) < len(columns):
+            raise ValueError("two parameters share a step count tensor: each needs its own")
+        self.values = list(chain.from_iterable(map(dict.values, opt.state.values())))
+        self.dtypes, self.numels = list(map(_dtype, self.params)), list(map(_numel, self.params))
+        self.tensors = self.params + [t for c in columns for t in c if t is not None]
+        self.at, self.grads_at = list(map(_ptr, self.tensors)), None
+        self.table = array("q", bytes(8 * _WORDS * len(chosen)))
+        for k, (p, c) in enumerate(zip(self.params, columns)):
+            self.table[k * _WORDS] = p.data_ptr()
+            for column, t in enumerate(c):
+                self.table[k * _WORDS + 2 + column] = 0 if t is None else t.data_ptr()
+        self.table[8::_WORDS] = array("q", self.numels)
+        self.table[9::_WORDS] = array("q", [_DTYPES[p.dtype] | group["state_bits"] << 32 for p, _, _, group in chosen])
+        self.table[10::_WORDS] = array("q", [i for _, _, i, _ in chosen])
+
+    @staticmethod
+    def _settings(groups):
+        return [(g["state_bits"], g["master"], len(g["params"])) for g in groups]
+
+    def holds(self, groups, params, grads, state):
+        """Whether this step takes the same parameters with the same state tensors in the same places."""
+        if (len(params) != len(self.every) or not all(map(is_, params, self.every))
+                or list(map(is_, grads, repeat(None))) != self.without or self._settings(groups) != self.settings):
+            return False
+        values = list(chain.from_iterable(map(dict.values, state.values())))
+        return (len(values) == len(self.values) and all(map(is_, values, self.values))
+                and list(map(_numel, self.params)) == self.numels
+                and list(map(_dtype, self.params)) == self.dtypes and all(map(_contiguous, self.params))
+                and list(map(_ptr, self.tensors)) == self.at)
+
+    def fill(self, grads):
+        """The table with the gradients' addresses, and the tensors that these are of."""
+        if len(grads) != len(self.params):
+            grads = [g for g in grads if g is not None]
+        if list(map(_dtype, grads)) != self.dtypes:
+            raise ValueError("a gradient must be of its parameter's type")
+        try:
+            contiguous = all(map(_contiguous, grads))
+        except RuntimeError:      # a sparse one: _dense says so
+            contiguous = False
+        if not contiguous:
+            grads = _dense(grads, self.device.index, "a gradient")
+        at = list(map(_ptr, grads))
+        if at != self.grads_at:
+            _dense(grads, self.device.index, "a gradient")
+            if list(map(_numel, grads)) != self.numels:
+                raise ValueError("a gradient must be of its parameter's size")
+            self.grads_at, self.table[1::_WORDS] = at, array("q", at)
+        return self.table, grads
 
 
 def clip_and_step(optimizer, params, max_norm: float) -> None:

@@ -819,9 +819,9 @@ def _list_call(device, call):
     """call(stream) with `device` current and its current stream (a list's tensors may live on
     another device than the current one)."""
     if device.index == torch.cuda.current_device():
-        return call(torch.cuda.current_stream().cuda_stream)
+        return call(torch._C._cuda_getCurrentRawStream(device.index))
     with torch.cuda.device(device):
-        return call(torch.cuda.current_stream().cuda_stream)
+        return call(torch._C._cuda_getCurrentRawStream(device.index))
 
 
 def list_norm(entries: array, device: torch.device) -> torch.Tensor:
