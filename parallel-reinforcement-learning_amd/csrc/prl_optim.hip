@@ -44,6 +44,14 @@ __device__ inline const PRL_GLOBAL T* gptr(const void* p) { return (const PRL_GL
 template <typename T>
 __device__ inline PRL_GLOBAL T* gptr(void* p) { return (PRL_GLOBAL T*)p; }
 
+// Everything a step touches is touched once: its loads and stores are marked nontemporal, so that they
+// pass the caches without displacing each other (126 M float32 values: 789 -> 679 us; loads alone
+// 761, stores alone 789).  The norm that goes before a step reads its gradients plainly: the step
+// then finds part of them in the Infinity Cache (nontemporal: 706 us); a norm by itself does not
+// (126 M bfloat16 values: plain 52 us, nontemporal 47.5).
+#define PRL_LOAD_NT(Q, p) __builtin_nontemporal_load((const PRL_GLOBAL Q*)(p))
+#define PRL_STORE_NT(Q, p, x) __builtin_nontemporal_store(x, (PRL_GLOBAL Q*)(p))
+
 // the batch's tensor that workgroup `b` works on: the last one whose first chunk is <= b
 __device__ inline int find_entry(const unsigned* start, int count, unsigned b) {
   int before = 0;
@@ -90,41 +98,71 @@ struct NormArgs {
 };
 static_assert(sizeof(NormArgs) <= 4096, "kernel arguments");
 
+// up to 4 values from x[0 .. left), zeros behind: the loads are issued together, then converted
 template <typename T>
-__device__ inline double norm_chunk(const void* px, int64_t lo, int64_t hi) {
-  const PRL_GLOBAL typename T::One* x = gptr<typename T::One>(px);
-  constexpr int U = 4;
-  double acc = 0.0;
-  int64_t i = lo + 4 * (int64_t)threadIdx.x;
-  for (; i + 4 * L_THREADS * (U - 1) + 4 <= hi; i += 4 * L_THREADS * U) {
-    typename T::Quad q[U];
+__device__ inline f32x4 load_part(const PRL_GLOBAL typename T::One* x, int left) {
+  typename T::One q[3] = {};
 #pragma unroll
-    for (int u = 0; u < U; ++u) q[u] = *(const PRL_GLOBAL typename T::Quad*)(x + i + 4 * L_THREADS * u);
+  for (int e = 0; e < 3; ++e)
+    if (e < left) q[e] = x[e];
+  return f32x4{T::widen1(q[0]), T::widen1(q[1]), T::widen1(q[2]), 0.0f};
+}
+template <typename T>
+__device__ inline void store_part(PRL_GLOBAL typename T::One* x, int left, f32x4 f) {
+#pragma unroll
+  for (int e = 0; e < 3; ++e)
+    if (e < left) x[e] = T::narrow1(f[e]);
+}
+
+template <typename T, bool ONCE>
+__device__ inline double norm_chunk(const void* px, int64_t lo, int64_t hi) {
+  typedef typename T::Quad Quad;
+  const PRL_GLOBAL typename T::One* x = gptr<typename T::One>(px);
+  constexpr int U = 16 / sizeof(Quad) * 4;   // 64 bytes in flight per thread
+  double acc = 0.0;
+  const auto add = [&](f32x4 f) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = fma((double)f[e], (double)f[e], acc);
+  };
+  int64_t base = lo;
+  for (; base + 4 * L_THREADS * U <= hi; base += 4 * L_THREADS * U) {
+    Quad q[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const f32x4 f = T::widen(q[u]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc = fma((double)f[e], (double)f[e], acc);
+      const PRL_GLOBAL typename T::One* at = x + base + 4 * (L_THREADS * u + (int)threadIdx.x);
+      if (ONCE) q[u] = PRL_LOAD_NT(Quad, at);
+      else q[u] = *(const PRL_GLOBAL Quad*)at;
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) add(T::widen(q[u]));
   }
-  for (; i < hi; i += 4 * L_THREADS)
-    for (int e = 0; e < 4; ++e)
-      if (i + e < hi) {
-        const double f = (double)T::widen1(x[i + e]);
-        acc = fma(f, f, acc);
-      }
+  if (base < hi) {
+    Quad q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = base + 4 * (L_THREADS * u + (int)threadIdx.x);
+      q[u] = Quad{};
+      if (i + 4 <= hi) q[u] = *(const PRL_GLOBAL Quad*)(x + i);
+    }
+    const int64_t part = hi & ~(int64_t)3;   // chunks start at multiples of 4
+    if (part < hi && threadIdx.x == 0) add(load_part<T>(x + part, (int)(hi - part)));
+#pragma unroll
+    for (int u = 0; u < U; ++u) add(T::widen(q[u]));
+  }
   return acc;
 }
 
+// ONCE: no step of the same gradients follows
+template <bool ONCE>
 __global__ __launch_bounds__(L_THREADS) void list_norm_kernel(const NormArgs a, double* partial) {
   __shared__ double s_part[L_THREADS / 64];
   const int e = find_entry(a.start, a.count, blockIdx.x);
   const int64_t n = a.n[e], lo = (int64_t)(blockIdx.x - a.start[e]) * a.chunk;
   const int64_t hi = lo + a.chunk < n ? lo + a.chunk : n;
   double acc;
-  if (a.dtype[e] == PRL_LIST_F32) acc = norm_chunk<F32>(a.x[e], lo, hi);
-  else if (a.dtype[e] == PRL_LIST_BF16) acc = norm_chunk<BF16>(a.x[e], lo, hi);
-  else acc = norm_chunk<F16>(a.x[e], lo, hi);
+  if (a.dtype[e] == PRL_LIST_F32) acc = norm_chunk<F32, ONCE>(a.x[e], lo, hi);
+  else if (a.dtype[e] == PRL_LIST_BF16) acc = norm_chunk<BF16, ONCE>(a.x[e], lo, hi);
+  else acc = norm_chunk<F16, ONCE>(a.x[e], lo, hi);
   acc = wave_sum_f64_to63(acc);
   if ((threadIdx.x & 63) == 63) s_part[threadIdx.x >> 6] = acc;
   __syncthreads();
@@ -211,7 +249,7 @@ struct Adam32Args {
 static_assert(sizeof(Adam32Args) <= 4096, "kernel arguments");
 
 __device__ inline float adam_weight(const Coef& c, float w, float m, float rms) {
-  return w * c.decay - c.step_size * (m / (rms * c.inv_bc2_sqrt + c.eps));
+  return w * c.decay - c.step_size * (m * __builtin_amdgcn_rcpf(rms * c.inv_bc2_sqrt + c.eps));
 }
 __device__ inline void adam_moments(const Coef& c, float g, float& m, float& v) {
   g = g * c.clip;
@@ -229,49 +267,56 @@ __device__ inline void adam32_chunk(const Coef& c, void* pp, const void* pg, flo
   PRL_GLOBAL float* v = gptr<float>(pv);
   typedef typename T::Quad Quad;
   constexpr int U = 2;
-  int64_t i = lo + 4 * (int64_t)threadIdx.x;
-  for (; i + 4 * L_THREADS * (U - 1) + 4 <= hi; i += 4 * L_THREADS * U) {
+  const auto step = [&](f32x4 gr, f32x4& x, f32x4& mq, f32x4& vq) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float me = mq[e], ve = vq[e];
+      adam_moments(c, gr[e], me, ve);
+      x[e] = adam_weight(c, x[e], me, sqrtf(ve));
+      mq[e] = me;
+      vq[e] = ve;
+    }
+  };
+  for (int64_t base = lo; base < hi; base += 4 * L_THREADS * U) {
     Quad pq[U], gq[U];
     f32x4 wq[U], mq[U], vq[U];
+    const int64_t k0 = base + 4 * (int)threadIdx.x;
+    const bool whole = base + 4 * L_THREADS * U <= hi;   // of the workgroup: no bounds in the usual case
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t k = i + 4 * L_THREADS * u;
-      if (MASTER) wq[u] = *(const PRL_GLOBAL f32x4_u*)(w + k);
-      else pq[u] = *(const PRL_GLOBAL Quad*)(p + k);
-      gq[u] = *(const PRL_GLOBAL Quad*)(g + k);
-      mq[u] = *(const PRL_GLOBAL f32x4_u*)(m + k);
-      vq[u] = *(const PRL_GLOBAL f32x4_u*)(v + k);
+      const int64_t k = k0 + 4 * L_THREADS * u;
+      if (whole || k + 4 <= hi) {
+        if (MASTER) wq[u] = PRL_LOAD_NT(f32x4_u, w + k);
+        else pq[u] = PRL_LOAD_NT(Quad, p + k);
+        gq[u] = PRL_LOAD_NT(Quad, g + k);
+        mq[u] = PRL_LOAD_NT(f32x4_u, m + k);
+        vq[u] = PRL_LOAD_NT(f32x4_u, v + k);
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t k = i + 4 * L_THREADS * u;
-      f32x4 x = MASTER ? wq[u] : T::widen(pq[u]);
-      const f32x4 gr = T::widen(gq[u]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float me = mq[u][e], ve = vq[u][e];
-        adam_moments(c, gr[e], me, ve);
-        x[e] = adam_weight(c, x[e], me, sqrtf(ve));
-        mq[u][e] = me;
-        vq[u][e] = ve;
+      const int64_t k = k0 + 4 * L_THREADS * u;
+      if (whole || k + 4 <= hi) {
+        f32x4 x = MASTER ? wq[u] : T::widen(pq[u]);
+        step(T::widen(gq[u]), x, mq[u], vq[u]);
+        PRL_STORE_NT(f32x4_u, m + k, mq[u]);
+        PRL_STORE_NT(f32x4_u, v + k, vq[u]);
+        if (MASTER) PRL_STORE_NT(f32x4_u, w + k, x);
+        PRL_STORE_NT(Quad, p + k, T::narrow(x));
       }
-      *(PRL_GLOBAL f32x4_u*)(m + k) = mq[u];
-      *(PRL_GLOBAL f32x4_u*)(v + k) = vq[u];
-      if (MASTER) *(PRL_GLOBAL f32x4_u*)(w + k) = x;
-      *(PRL_GLOBAL Quad*)(p + k) = T::narrow(x);
     }
   }
-  for (; i < hi; i += 4 * L_THREADS)
-    for (int e = 0; e < 4; ++e)
-      if (i + e < hi) {
-        float me = m[i + e], ve = v[i + e];
-        adam_moments(c, T::widen1(g[i + e]), me, ve);
-        const float x = adam_weight(c, MASTER ? w[i + e] : T::widen1(p[i + e]), me, sqrtf(ve));
-        m[i + e] = me;
-        v[i + e] = ve;
-        if (MASTER) w[i + e] = x;
-        p[i + e] = T::narrow1(x);
-      }
+  const int64_t part = hi & ~(int64_t)3;   // a tensor's last 1 .. 3 values: one thread's
+  if (part < hi && threadIdx.x == L_THREADS - 1) {
+    const int left = (int)(hi - part);
+    f32x4 gr = load_part<T>(g + part, left), mq = load_part<F32>(m + part, left), vq = load_part<F32>(v + part, left);
+    f32x4 x = MASTER ? load_part<F32>(w + part, left) : load_part<T>(p + part, left);
+    step(gr, x, mq, vq);
+    store_part<F32>(m + part, left, mq);
+    store_part<F32>(v + part, left, vq);
+    if (MASTER) store_part<F32>(w + part, left, x);
+    store_part<T>(p + part, left, x);
+  }
 }
 
 __global__ __launch_bounds__(L_THREADS) void list_adam32_kernel(const Adam32Args a) {
@@ -300,8 +345,8 @@ struct Adam8Args {
   void* param[L_BATCH8];
   const void* grad[L_BATCH8];
   float* master[L_BATCH8];
-  unsigned* m[L_BATCH8];
-  unsigned* r[L_BATCH8];
+  void* m[L_BATCH8];
+  void* r[L_BATCH8];
   float* m_scale[L_BATCH8];
   float* r_scale[L_BATCH8];
   int64_t n[L_BATCH8];
@@ -325,127 +370,140 @@ __device__ inline unsigned wave_max_u32(unsigned x) {
   return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
 }
 
-// two 16-bit draws for value i of a tensor at this step
-__device__ inline unsigned draw_bits(int64_t i, unsigned seed) {
-  unsigned h = ((unsigned)i + (unsigned)((uint64_t)i >> 32) * 0x85EBCA77u) ^ seed;
+// a value's two 16-bit draws at this step are the halves of h ^ (h >> 16), h = draw_bits(its index
+// folded to 32 bits, ..): the low one for the first moment, the high one for the second
+__device__ inline unsigned draw_bits(unsigned at, unsigned seed) {
+  unsigned h = at ^ seed;
   h = (h ^ (h >> 16)) * 0x7FEB352Du;
   h = (h ^ (h >> 15)) * 0x846CA68Bu;
-  return h ^ (h >> 16);
+  asm("" : "+v"(h));   // opaque: the compiler would form h << 16 by a third multiplication (quarter rate)
+  return h;
 }
 
-// y in [0, 256] to a neighbour on the e4m3 grid: adding 20 random bits below the 3 mantissa bits
-// kept and truncating goes up with probability = the way past the lower neighbour.  Below the
-// smallest normal value the grid is even with the step of the first binade, so y moves there.
-__device__ inline float round_e4m3(float y, unsigned draw16) {
-  const float shift = y < 0x1p-6f ? 0x1p-6f : 0.0f;
-  const unsigned u = (__float_as_uint(y + shift) + (draw16 << 4)) & 0xFFF00000u;
-  return __uint_as_float(u) - shift;
-}
-
-struct Scale {
-  float k, store;   // 256 / A (0: the block is held as zeros), and A as stored
-};
-__device__ inline Scale block_scale(unsigned max_bits) {
+// 256 / A for a block's largest magnitude A given as its bits; 0: the block is held as zeros
+__device__ inline float block_factor(unsigned max_bits) {
   const float A = __uint_as_float(max_bits);
-  Scale s;
-  s.k = 0.0f;
-  s.store = 0.0f;
-  if (max_bits >= 0x7f800000u) s.store = __uint_as_float(0x7fc00000u);
-  else if (A >= 0x1p-118f) {
-    s.k = 256.0f / A;
-    s.store = A;
-  }
-  return s;
+  return max_bits < 0x7f800000u && A >= 0x1p-118f ? 256.0f / A : 0.0f;
+}
+// A as stored: NaN where a value of the block is not finite
+__device__ inline float block_store(unsigned max_bits, float k) {
+  return max_bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : k > 0.0f ? __uint_as_float(max_bits) : 0.0f;
 }
 
-template <typename T, bool MASTER>
-__device__ inline void adam8_block(const Coef& c, void* pp, const void* pg, float* pw, unsigned* pm,
-                                   unsigned* pr, float* pms, float* prs, int64_t base, int64_t n) {
+// The pointers are the block's own (uniform over the wave); left: its values, 256 but for a tensor's
+// last block (WHOLE: known to be 256); at: the first value's index folded to 32 bits.
+template <typename T, bool MASTER, bool WHOLE>
+__device__ inline void adam8_block(const Coef& c, PRL_GLOBAL typename T::One* p, const PRL_GLOBAL typename T::One* g,
+                                   PRL_GLOBAL float* w, PRL_GLOBAL unsigned char* mc, PRL_GLOBAL unsigned char* rc,
+                                   PRL_GLOBAL float* ms, PRL_GLOBAL float* rs, unsigned at, int left) {
   typedef typename T::Quad Quad;
-  const int64_t i = base + 4 * (int64_t)(threadIdx.x & 63), b = base / PRL_LIST_BLOCK;
-  PRL_GLOBAL typename T::One* p = gptr<typename T::One>(pp) + i;
-  const PRL_GLOBAL typename T::One* g = gptr<typename T::One>(pg) + i;
-  PRL_GLOBAL float* w = gptr<float>(pw) + (MASTER ? i : 0);
-  PRL_GLOBAL unsigned char* mc = gptr<unsigned char>((void*)pm) + i;
-  PRL_GLOBAL unsigned char* rc = gptr<unsigned char>((void*)pr) + i;
-  const bool whole = i + 4 <= n;
-  const int left = whole ? 4 : (i < n ? (int)(n - i) : 0);
-  f32x4 x = {0.f, 0.f, 0.f, 0.f}, gr = x;
+  const int lane = threadIdx.x & 63;
+  const unsigned i = 4 * lane;
+  left = WHOLE ? 4 : left - (int)i;   // this lane's values: 4 or more, 1 .. 3, or none
+  f32x4 x, gr;
   unsigned mq = 0, rq = 0;
-  if (whole) {
-    gr = T::widen(*(const PRL_GLOBAL Quad*)g);
-    x = MASTER ? *(const PRL_GLOBAL f32x4_u*)w : T::widen(*(const PRL_GLOBAL Quad*)p);
-    mq = *(const PRL_GLOBAL u32_u*)mc;
-    rq = *(const PRL_GLOBAL u32_u*)rc;
+  if (left >= 4) {
+    gr = T::widen(PRL_LOAD_NT(Quad, g + i));
+    if (MASTER) x = PRL_LOAD_NT(f32x4_u, w + i);
+    else x = T::widen(PRL_LOAD_NT(Quad, p + i));
+    mq = PRL_LOAD_NT(u32_u, mc + i);
+    rq = PRL_LOAD_NT(u32_u, rc + i);
   } else {
+    gr = load_part<T>(g + i, left);
+    x = MASTER ? load_part<F32>(w + i, left) : load_part<T>(p + i, left);
     for (int e = 0; e < 3; ++e)
       if (e < left) {
-        gr[e] = T::widen1(g[e]);
-        x[e] = MASTER ? w[e] : T::widen1(p[e]);
-        mq |= (unsigned)mc[e] << (8 * e);
-        rq |= (unsigned)rc[e] << (8 * e);
+        mq |= (unsigned)mc[i + e] << (8 * e);
+        rq |= (unsigned)rc[i + e] << (8 * e);
       }
   }
-  const float ms = gptr<float>(pms)[b] * 0x1p-8f, rs = gptr<float>(prs)[b] * 0x1p-8f;
+  const float ma = ms[0] * 0x1p-8f, ra = rs[0] * 0x1p-8f;
   float m[4] = {__builtin_amdgcn_cvt_f32_fp8(mq, 0), __builtin_amdgcn_cvt_f32_fp8(mq, 1),
                 __builtin_amdgcn_cvt_f32_fp8(mq, 2), __builtin_amdgcn_cvt_f32_fp8(mq, 3)};
   float r[4] = {__builtin_amdgcn_cvt_f32_fp8(rq, 0), __builtin_amdgcn_cvt_f32_fp8(rq, 1),
                 __builtin_amdgcn_cvt_f32_fp8(rq, 2), __builtin_amdgcn_cvt_f32_fp8(rq, 3)};
-  unsigned m_max = 0, r_max = 0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    m[e] = m[e] * ms;
-    r[e] = r[e] * rs;
+    m[e] = m[e] * ma;
+    r[e] = r[e] * ra;
     float v = r[e] * r[e];
     adam_moments(c, gr[e], m[e], v);
     r[e] = sqrtf(v);
-    if (e >= left) m[e] = r[e] = 0.0f;   // past the tensor's end (a NaN scale or clip must not count twice)
-    const unsigned mb = __float_as_uint(m[e]) & 0x7fffffffu, rb = __float_as_uint(r[e]) & 0x7fffffffu;
+    x[e] = adam_weight(c, x[e], m[e], r[e]);
+    if (!WHOLE && e >= left) m[e] = r[e] = 0.0f;   // past the tensor's end nothing counts (a NaN clip would)
+  }
+  if (left >= 4) {
+    if (MASTER) PRL_STORE_NT(f32x4_u, w + i, x);
+    PRL_STORE_NT(Quad, p + i, T::narrow(x));
+  } else {
+    if (MASTER) store_part<F32>(w + i, left, x);
+    store_part<T>(p + i, left, x);
+  }
+  unsigned m_max = 0, r_max = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const unsigned mb = __float_as_uint(m[e]) & 0x7fffffffu, rb = __float_as_uint(r[e]);   // r >= 0 or NaN
     m_max = m_max > mb ? m_max : mb;
     r_max = r_max > rb ? r_max : rb;
   }
-  const Scale sm = block_scale(wave_max_u32(m_max)), sr = block_scale(wave_max_u32(r_max));
-  float mo[4], ro[4];
+  m_max = wave_max_u32(m_max);
+  r_max = wave_max_u32(r_max);
+  // both factors in one division: the first moment's in lane 0, the second's in lane 1
+  const float k = block_factor(lane & 1 ? r_max : m_max);
+  const float km = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(k), 0));
+  const float kr = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(k), 1));
+  // stochastic rounding to e4m3: the conversion adds its random bits below the mantissa bits it keeps
+  // and truncates, the sign aside; 16 of the 20 are drawn, the rest are 0
+  unsigned d[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    x[e] = adam_weight(c, x[e], m[e], r[e]);
-    const unsigned d = draw_bits(i + e, c.seed);
-    // k == 0: zeros (a product with a NaN or an infinity would not be)
-    const float ym = sm.k > 0.0f ? fminf(fabsf(m[e]) * sm.k, 256.0f) : 0.0f;
-    const float yr = sr.k > 0.0f ? fminf(r[e] * sr.k, 256.0f) : 0.0f;
-    mo[e] = copysignf(round_e4m3(ym, d & 0xffffu), m[e]);
-    ro[e] = round_e4m3(yr, d >> 16);
-    if (r[e] > 0.0f && sr.k > 0.0f) ro[e] = fmaxf(ro[e], 0x1p-9f);
+  for (int e = 0; e < 4; ++e) d[e] = draw_bits(at + i + e, c.seed);
+  int mw = 0, rw = 0;
+  if (km > 0.0f) {
+    const auto y = [&](int e) { return __builtin_amdgcn_fmed3f(m[e] * km, -256.0f, 256.0f); };
+    const auto draw = [&](int e) { return (d[e] << 16) ^ (d[e] & 0xffff0000u); };
+    mw = __builtin_amdgcn_cvt_sr_fp8_f32(y(0), draw(0), mw, 0);
+    mw = __builtin_amdgcn_cvt_sr_fp8_f32(y(1), draw(1), mw, 1);
+    mw = __builtin_amdgcn_cvt_sr_fp8_f32(y(2), draw(2), mw, 2);
+    mw = __builtin_amdgcn_cvt_sr_fp8_f32(y(3), draw(3), mw, 3);
   }
-  int mw = __builtin_amdgcn_cvt_pk_fp8_f32(mo[0], mo[1], 0, false);
-  mw = __builtin_amdgcn_cvt_pk_fp8_f32(mo[2], mo[3], mw, true);
-  int rw = __builtin_amdgcn_cvt_pk_fp8_f32(ro[0], ro[1], 0, false);
-  rw = __builtin_amdgcn_cvt_pk_fp8_f32(ro[2], ro[3], rw, true);
-  if (whole) {
-    if (MASTER) *(PRL_GLOBAL f32x4_u*)w = x;
-    *(PRL_GLOBAL Quad*)p = T::narrow(x);
-    *(PRL_GLOBAL u32_u*)mc = (unsigned)mw;
-    *(PRL_GLOBAL u32_u*)rc = (unsigned)rw;
+  if (kr > 0.0f) {   // an r above 0 stays above 0: 2^-9 is the smallest code
+    const auto y = [&](int e) { return r[e] > 0.0f ? __builtin_amdgcn_fmed3f(r[e] * kr, 0x1p-9f, 256.0f) : 0.0f; };
+    const auto draw = [&](int e) { return d[e] & 0xffff0000u; };
+    rw = __builtin_amdgcn_cvt_sr_fp8_f32(y(0), draw(0), rw, 0);
+    rw = __builtin_amdgcn_cvt_sr_fp8_f32(y(1), draw(1), rw, 1);
+    rw = __builtin_amdgcn_cvt_sr_fp8_f32(y(2), draw(2), rw, 2);
+    rw = __builtin_amdgcn_cvt_sr_fp8_f32(y(3), draw(3), rw, 3);
+  }
+  if (left >= 4) {
+    PRL_STORE_NT(u32_u, mc + i, (unsigned)mw);
+    PRL_STORE_NT(u32_u, rc + i, (unsigned)rw);
   } else {
     for (int e = 0; e < 3; ++e)
       if (e < left) {
-        if (MASTER) w[e] = x[e];
-        p[e] = T::narrow1(x[e]);
-        mc[e] = (unsigned char)((unsigned)mw >> (8 * e));
-        rc[e] = (unsigned char)((unsigned)rw >> (8 * e));
+        mc[i + e] = (unsigned char)((unsigned)mw >> (8 * e));
+        rc[i + e] = (unsigned char)((unsigned)rw >> (8 * e));
       }
   }
-  if ((threadIdx.x & 63) == 0) {
-    gptr<float>(pms)[b] = sm.store;
-    gptr<float>(prs)[b] = sr.store;
+  if (lane == 0) {
+    ms[0] = block_store(m_max, km);
+    rs[0] = block_store(r_max, kr);
   }
 }
 
 template <typename T, bool MASTER>
 __device__ inline void adam8_chunk(const Coef& c, const Adam8Args& a, int e, int64_t lo, int64_t hi, int64_t n) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  for (int64_t base = lo + wave * PRL_LIST_BLOCK; base < hi; base += L_THREADS / 64 * PRL_LIST_BLOCK)
-    adam8_block<T, MASTER>(c, a.param[e], a.grad[e], a.master[e], a.m[e], a.r[e], a.m_scale[e], a.r_scale[e], base, n);
+  for (int64_t base = lo + wave * PRL_LIST_BLOCK; base < hi; base += L_THREADS / 64 * PRL_LIST_BLOCK) {
+    const int64_t b = base / PRL_LIST_BLOCK;
+    const unsigned at = (unsigned)base + (unsigned)((uint64_t)base >> 32) * 0x85EBCA77u;
+    PRL_GLOBAL typename T::One* p = gptr<typename T::One>(a.param[e]) + base;
+    const PRL_GLOBAL typename T::One* g = gptr<typename T::One>(a.grad[e]) + base;
+    PRL_GLOBAL float* w = gptr<float>(a.master[e]) + (MASTER ? base : 0);
+    PRL_GLOBAL unsigned char *mc = gptr<unsigned char>(a.m[e]) + base, *rc = gptr<unsigned char>(a.r[e]) + base;
+    PRL_GLOBAL float *ms = gptr<float>(a.m_scale[e]) + b, *rs = gptr<float>(a.r_scale[e]) + b;
+    if (base + PRL_LIST_BLOCK <= n) adam8_block<T, MASTER, true>(c, p, g, w, mc, rc, ms, rs, at, PRL_LIST_BLOCK);
+    else adam8_block<T, MASTER, false>(c, p, g, w, mc, rc, ms, rs, at, (int)(n - base));
+  }
 }
 
 __global__ __launch_bounds__(L_THREADS) void list_adam8_kernel(const Adam8Args a) {
@@ -473,14 +531,15 @@ inline int64_t list_total(const prl_list_entry* e, int64_t count) {
 }
 
 // the partial sums of all grads' squares into partial[0 .. *n_partial)
-int launch_norm(const prl_list_entry* e, int64_t count, double* partial, int64_t* n_partial, hipStream_t st) {
+int launch_norm(const prl_list_entry* e, int64_t count, bool once, double* partial, int64_t* n_partial, hipStream_t st) {
   const int64_t tile = 4 * L_THREADS * 4;
   NormArgs a{};
   a.chunk = tile * (1 + list_total(e, count) / (tile * L_NORM_BLOCKS));
   int64_t done = 0, blocks = 0;
   for (int64_t i = 0; i <= count; ++i) {
     if (a.count == L_BATCH || (i == count && a.count > 0)) {
-      hipLaunchKernelGGL(list_norm_kernel, dim3((unsigned)blocks), dim3(L_THREADS), 0, st, a, partial + done);
+      if (once) hipLaunchKernelGGL(list_norm_kernel<true>, dim3((unsigned)blocks), dim3(L_THREADS), 0, st, a, partial + done);
+      else hipLaunchKernelGGL(list_norm_kernel<false>, dim3((unsigned)blocks), dim3(L_THREADS), 0, st, a, partial + done);
       PRL_LAUNCH_CHECK("list_norm");
       done += blocks;
       blocks = 0;
@@ -576,8 +635,8 @@ int launch_adam8(const prl_list_entry* e, int64_t count, const Coef* coef, hipSt
     a.param[k] = e[i].param;
     a.grad[k] = e[i].grad;
     a.master[k] = e[i].master;
-    a.m[k] = static_cast<unsigned*>(e[i].exp_avg);
-    a.r[k] = static_cast<unsigned*>(e[i].second);
+    a.m[k] = e[i].exp_avg;
+    a.r[k] = e[i].second;
     a.m_scale[k] = e[i].exp_avg_scale;
     a.r_scale[k] = e[i].second_scale;
     a.n[k] = e[i].numel;
@@ -625,7 +684,7 @@ extern "C" int prl_list_norm(const prl_list_entry* entries, int64_t count, float
   Coef* coef = static_cast<Coef*>(workspace);
   double* partial = reinterpret_cast<double*>(coef + count);
   int64_t n_partial = 0;
-  if (int rc = launch_norm(entries, count, partial, &n_partial, as_stream(stream))) return rc;
+  if (int rc = launch_norm(entries, count, true, partial, &n_partial, as_stream(stream))) return rc;
   return launch_begin(entries, 0, nullptr, 0.0f, norm, partial, n_partial, coef, as_stream(stream));
 }
 
@@ -661,7 +720,7 @@ extern "C" int prl_list_adamw(const prl_list_entry* entries, int64_t count, cons
   double* partial = reinterpret_cast<double*>(coef + count);
   int64_t n_partial = 0;
   if (norm) {
-    if (int rc = launch_norm(entries, count, partial, &n_partial, st)) return rc;
+    if (int rc = launch_norm(entries, count, false, partial, &n_partial, st)) return rc;
   }
   if (int rc = launch_begin(entries, count, groups, max_norm, norm, partial, n_partial, coef, st)) return rc;
   if (int rc = launch_adam32(entries, count, coef, st)) return rc;

@@ -70,10 +70,10 @@ def step64(w, g, m, v, t, lr, betas, eps, wd, c):
     # products and a sum of positive terms: c twice (6 U) + its products (2) + square, coefficients,
     # products, sum (4): at most 12 U of the result; the smallest steps of a float32 below 2^-126
     ev = 12 * U32 * v1 + 2.0 ** -148
-    # the quotient takes m's error, half of v's (a root), and its own roundings: root, two
-    # coefficients, product, sum, quotient, step size, product (8 U); then the decayed weight (3 U)
-    # and the sum
+    # the quotient takes m's error, half of v's (a root), and its own roundings: root, two coefficients,
+    # product, sum, the reciprocal (1 ulp: 2 U), two products (9 U); then the decayed weight (3 U) and
+    # the sum
     part = step_size * m1.abs() / denom
-    ew = (step_size * em / denom + (6 + 8) * U32 * part + step_size * m1.abs() / denom ** 2 * 2.0 ** -74
+    ew = (step_size * em / denom + (6 + 9) * U32 * part + step_size * m1.abs() / denom ** 2 * 2.0 ** -74
           + 3 * U32 * w.abs() + U32 * w1.abs())
     return w1, m1, v1, ew, em, ev
