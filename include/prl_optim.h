@@ -47,9 +47,10 @@ typedef struct prl_list_group {   /* host */
                            graph then follows a schedule) */
 } prl_list_group;
 
-/* Workspace of the two calls below for `count` tensors.  It holds nothing between calls and needs
- * no initial value; two calls that may run at once need one each. */
-int64_t prl_list_workspace_bytes(int64_t count);
+/* Workspace of the two calls below for a list of these sizes (prl_list_norm: n_groups 0); 0 for a
+ * short list, which needs none (NULL will do); -1 for a list that they refuse.  It holds nothing
+ * between calls and needs no initial value; two calls that may run at once need one each. */
+int64_t prl_list_workspace_bytes(const prl_list_entry* entries, int64_t count, int64_t n_groups);
 
 /* *norm = sqrt(sum over the tensors' grads of their squares), summed in float64 in a fixed order. */
 int prl_list_norm(const prl_list_entry* entries, int64_t count, float* norm, void* workspace,

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import struct
 from array import array
+from importlib import import_module
 from itertools import chain, repeat
 from operator import attrgetter, is_
 
@@ -29,6 +30,10 @@ _MOMENTS = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_rms", "exp_avg_sc
 _ptr, _numel, _contiguous, _device = (torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous,
                                       torch.Tensor.get_device)
 _dtype, _layout = attrgetter("dtype"), attrgetter("layout")
+
+
+_GLOBAL_HOOKS = [getattr(import_module("torch.optim.optimizer"), f"_global_optimizer_{k}_hooks", (True,))
+                 for k in ("pre", "post")]
 
 
 def _dense(tensors, device, name):
@@ -186,6 +191,20 @@ class AdamW(torch.optim.Optimizer):
     def step(self, closure=None, *, max_norm=None):
         """One step of every parameter that has a gradient; with max_norm (>= 0) the gradients of
         all groups are clipped together by their global norm first (p.grad stays as it is)."""
+        if (self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or any(_GLOBAL_HOOKS)
+                or torch.autograd._profiler_enabled()):
+            return self._traced_step(closure, max_norm=max_norm)
+        return self._step(closure, max_norm)
+
+    # torch wraps an optimizer's step() to run its hooks and mark it for the profiler, some 5 us; this
+    # one goes through that wrapper when there is a hook to run or a profiler to see the mark
+    step.hooked = True
+
+    @torch.optim.Optimizer.profile_hook_step
+    def _traced_step(self, closure=None, *, max_norm=None):
+        return self._step(closure, max_norm)
+
+    def _step(self, closure, max_norm):
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -206,7 +225,7 @@ class AdamW(torch.optim.Optimizer):
         words = b"".join(map(self._group_words, groups))
         table, keep = plan.fill(grads)
         self.total_norm = prl_native.list_adamw(table, array("q", words), plan.device,
-                                                None if max_norm is None else float(max_norm))
+                                                None if max_norm is None else float(max_norm), plan.workspace)
         return loss
 
     @staticmethod
@@ -262,6 +281,7 @@ class _Plan:
         self.table[8::_WORDS] = array("q", self.numels)
         self.table[9::_WORDS] = array("q", [_DTYPES[p.dtype] | group["state_bits"] << 32 for p, _, _, group in chosen])
         self.table[10::_WORDS] = array("q", [i for _, _, i, _ in chosen])
+        self.workspace = prl_native.list_workspace_bytes(self.table, len(groups))
 
     @staticmethod
     def _settings(groups):

@@ -4,7 +4,9 @@
 // The tensors' descriptors travel in the kernels' arguments, a batch of up to 64 tensors per launch:
 // a captured graph then holds them itself, and no table on the device has to outlive a call.  Every
 // tensor is cut into chunks of one workgroup each; a workgroup finds its tensor by comparing its
-// index with the batch's chunk prefix, 64 entries per ballot.
+// index with the batch's chunk prefix, 64 entries per ballot.  Fields that a uniform index reads
+// from the arguments are 4 or 8 bytes wide: of a byte array and a pointer array with one index the
+// compiler once formed a scalar load from two unaligned parts, whose low bits the hardware drops.
 //
 // One call: list_norm_kernel (per batch; one float64 partial sum per chunk), then list_begin_kernel
 // (one workgroup: folds the partials into the norm and the clip coefficient, advances every
@@ -92,7 +94,7 @@ struct NormArgs {
   const void* x[L_BATCH];
   int64_t n[L_BATCH];
   unsigned start[L_BATCH];
-  unsigned char dtype[L_BATCH];
+  unsigned dtype[L_BATCH];
   int64_t chunk;
   int count;
 };
@@ -173,6 +175,29 @@ __global__ __launch_bounds__(L_THREADS) void list_norm_kernel(const NormArgs a, 
   }
 }
 
+// ---- the clip coefficient, and a tensor's scalars --------------------------------------------------
+__device__ inline float clip_coef(float norm, float max_norm) {
+  const float clip = max_norm / (norm + 1e-6f);
+  return clip > 1.0f ? 1.0f : clip;   // a NaN stays
+}
+// advances the step count
+__device__ inline Coef next_coef(const prl_list_group& g, float* count, float clip) {
+  const double lr = g.lr_dev != nullptr ? (double)g.lr_dev[0] : g.lr;
+  const float step = count[0] + 1.0f;
+  count[0] = step;
+  Coef c{};
+  c.clip = clip;
+  c.decay = (float)(1.0 - lr * g.weight_decay);
+  c.step_size = (float)(lr / (1.0 - pow(g.beta1, (double)step)));
+  c.inv_bc2_sqrt = (float)(1.0 / sqrt(1.0 - pow(g.beta2, (double)step)));
+  c.omb1 = (float)(1.0 - g.beta1);
+  c.omb2 = (float)(1.0 - g.beta2);
+  c.beta2 = (float)g.beta2;
+  c.eps = (float)g.eps;
+  c.seed = (unsigned)(int64_t)step * 0x9E3779B1u;
+  return c;
+}
+
 // ---- once per call: the norm's fold, the step counts, the per-tensor scalars -------------------
 struct BeginArgs {
   float* step[L_BATCH_BEGIN];
@@ -210,26 +235,8 @@ __global__ __launch_bounds__(1024) void list_begin_kernel(const BeginArgs a) {
     __syncthreads();
   }
   if (t >= a.count) return;
-  float clip = 1.0f;
-  if (a.norm != nullptr) {
-    clip = a.max_norm / (s_norm + 1e-6f);
-    if (clip > 1.0f) clip = 1.0f;   // a NaN stays
-  }
-  const prl_list_group& g = a.groups[a.group[t]];
-  const double lr = g.lr_dev != nullptr ? (double)g.lr_dev[0] : g.lr;
-  const float step = a.step[t][0] + 1.0f;
-  a.step[t][0] = step;
-  Coef c{};
-  c.clip = clip;
-  c.decay = (float)(1.0 - lr * g.weight_decay);
-  c.step_size = (float)(lr / (1.0 - pow(g.beta1, (double)step)));
-  c.inv_bc2_sqrt = (float)(1.0 / sqrt(1.0 - pow(g.beta2, (double)step)));
-  c.omb1 = (float)(1.0 - g.beta1);
-  c.omb2 = (float)(1.0 - g.beta2);
-  c.beta2 = (float)g.beta2;
-  c.eps = (float)g.eps;
-  c.seed = (unsigned)(int64_t)step * 0x9E3779B1u;
-  a.coef[t] = c;
+  const float clip = a.norm != nullptr ? clip_coef(s_norm, a.max_norm) : 1.0f;
+  a.coef[t] = next_coef(a.groups[a.group[t]], a.step[t], clip);
 }
 
 // ---- the step, 32-bit moments ------------------------------------------------------------------
@@ -257,6 +264,30 @@ __device__ inline void adam_moments(const Coef& c, float g, float& m, float& v) 
   v = v * c.beta2 + (g * g) * c.omb2;
 }
 
+__device__ inline void adam32_quad(const Coef& c, f32x4 g, f32x4& x, f32x4& m, f32x4& v) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float me = m[e], ve = v[e];
+    adam_moments(c, g[e], me, ve);
+    x[e] = adam_weight(c, x[e], me, sqrtf(ve));
+    m[e] = me;
+    v[e] = ve;
+  }
+}
+// 1 .. 3 values
+template <typename T, bool MASTER>
+__device__ inline void adam32_part(const Coef& c, PRL_GLOBAL typename T::One* p, const PRL_GLOBAL typename T::One* g,
+                                   PRL_GLOBAL float* w, PRL_GLOBAL float* m, PRL_GLOBAL float* v, int left) {
+  const f32x4 gr = load_part<T>(g, left);
+  f32x4 mq = load_part<F32>(m, left), vq = load_part<F32>(v, left);
+  f32x4 x = MASTER ? load_part<F32>(w, left) : load_part<T>(p, left);
+  adam32_quad(c, gr, x, mq, vq);
+  store_part<F32>(m, left, mq);
+  store_part<F32>(v, left, vq);
+  if (MASTER) store_part<F32>(w, left, x);
+  store_part<T>(p, left, x);
+}
+
 template <typename T, bool MASTER>
 __device__ inline void adam32_chunk(const Coef& c, void* pp, const void* pg, float* pw, float* pm,
                                     float* pv, int64_t lo, int64_t hi) {
@@ -267,16 +298,6 @@ __device__ inline void adam32_chunk(const Coef& c, void* pp, const void* pg, flo
   PRL_GLOBAL float* v = gptr<float>(pv);
   typedef typename T::Quad Quad;
   constexpr int U = 2;
-  const auto step = [&](f32x4 gr, f32x4& x, f32x4& mq, f32x4& vq) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float me = mq[e], ve = vq[e];
-      adam_moments(c, gr[e], me, ve);
-      x[e] = adam_weight(c, x[e], me, sqrtf(ve));
-      mq[e] = me;
-      vq[e] = ve;
-    }
-  };
   for (int64_t base = lo; base < hi; base += 4 * L_THREADS * U) {
     Quad pq[U], gq[U];
     f32x4 wq[U], mq[U], vq[U];
@@ -298,7 +319,7 @@ __device__ inline void adam32_chunk(const Coef& c, void* pp, const void* pg, flo
       const int64_t k = k0 + 4 * L_THREADS * u;
       if (whole || k + 4 <= hi) {
         f32x4 x = MASTER ? wq[u] : T::widen(pq[u]);
-        step(T::widen(gq[u]), x, mq[u], vq[u]);
+        adam32_quad(c, T::widen(gq[u]), x, mq[u], vq[u]);
         PRL_STORE_NT(f32x4_u, m + k, mq[u]);
         PRL_STORE_NT(f32x4_u, v + k, vq[u]);
         if (MASTER) PRL_STORE_NT(f32x4_u, w + k, x);
@@ -307,16 +328,8 @@ __device__ inline void adam32_chunk(const Coef& c, void* pp, const void* pg, flo
     }
   }
   const int64_t part = hi & ~(int64_t)3;   // a tensor's last 1 .. 3 values: one thread's
-  if (part < hi && threadIdx.x == L_THREADS - 1) {
-    const int left = (int)(hi - part);
-    f32x4 gr = load_part<T>(g + part, left), mq = load_part<F32>(m + part, left), vq = load_part<F32>(v + part, left);
-    f32x4 x = MASTER ? load_part<F32>(w + part, left) : load_part<T>(p + part, left);
-    step(gr, x, mq, vq);
-    store_part<F32>(m + part, left, mq);
-    store_part<F32>(v + part, left, vq);
-    if (MASTER) store_part<F32>(w + part, left, x);
-    store_part<T>(p + part, left, x);
-  }
+  if (part < hi && threadIdx.x == L_THREADS - 1)
+    adam32_part<T, MASTER>(c, p + part, g + part, w + (MASTER ? part : 0), m + part, v + part, (int)(hi - part));
 }
 
 __global__ __launch_bounds__(L_THREADS) void list_adam32_kernel(const Adam32Args a) {
@@ -523,6 +536,130 @@ __global__ __launch_bounds__(L_THREADS) void list_adam8_kernel(const Adam8Args a
   }
 }
 
+// ---- a short list in one launch ------------------------------------------------------------------
+// Up to L_SMALL_ITEMS blocks of 256 values in L_SMALL tensors: one workgroup of 16 waves, a block per
+// wave at a time, takes the norm, the scalars and the step.  Such a list's time is the launches'.
+constexpr int L_SMALL = 32;
+constexpr int L_SMALL_ITEMS = 160;
+constexpr int L_SMALL_WAVES = 16;
+struct SmallArgs {
+  void* param[L_SMALL];
+  const void* grad[L_SMALL];
+  float* master[L_SMALL];
+  void* m[L_SMALL];
+  void* r[L_SMALL];
+  float* m_scale[L_SMALL];
+  float* r_scale[L_SMALL];
+  float* step[L_SMALL];
+  int n[L_SMALL];
+  unsigned start[L_SMALL];
+  unsigned kind[L_SMALL];    // dtype | bits << 8 | group << 16
+  prl_list_group groups[L_GROUPS];
+  float* norm;
+  float max_norm;
+  int count, items;
+};
+static_assert(sizeof(SmallArgs) <= 4096, "kernel arguments");
+
+template <typename T>
+__device__ inline f32x4 load_quad(const void* px, int i, int left) {
+  const PRL_GLOBAL typename T::One* x = gptr<typename T::One>(px) + i;
+  return left >= 4 ? T::widen(*(const PRL_GLOBAL typename T::Quad*)x) : load_part<T>(x, left);
+}
+
+template <typename T, bool MASTER>
+__device__ inline void small_item(const Coef& c, const SmallArgs& a, int e, int base) {
+  PRL_GLOBAL typename T::One* p = gptr<typename T::One>(a.param[e]) + base;
+  const PRL_GLOBAL typename T::One* g = gptr<typename T::One>(a.grad[e]) + base;
+  PRL_GLOBAL float* w = gptr<float>(a.master[e]) + (MASTER ? base : 0);
+  const int left = a.n[e] - base;
+  if ((a.kind[e] >> 8 & 0xff) == 8) {
+    PRL_GLOBAL unsigned char *mc = gptr<unsigned char>(a.m[e]) + base, *rc = gptr<unsigned char>(a.r[e]) + base;
+    PRL_GLOBAL float* ms = gptr<float>(a.m_scale[e]) + base / PRL_LIST_BLOCK;
+    PRL_GLOBAL float* rs = gptr<float>(a.r_scale[e]) + base / PRL_LIST_BLOCK;
+    adam8_block<T, MASTER, false>(c, p, g, w, mc, rc, ms, rs, (unsigned)base, left);
+    return;
+  }
+  PRL_GLOBAL float *m = gptr<float>(a.m[e]) + base, *v = gptr<float>(a.r[e]) + base;
+  const int i = 4 * (int)(threadIdx.x & 63);
+  if (i + 4 <= left) {
+    f32x4 mq = *(const PRL_GLOBAL f32x4_u*)(m + i), vq = *(const PRL_GLOBAL f32x4_u*)(v + i);
+    const f32x4 gr = T::widen(*(const PRL_GLOBAL typename T::Quad*)(g + i));
+    f32x4 x;
+    if (MASTER) x = *(const PRL_GLOBAL f32x4_u*)(w + i);
+    else x = T::widen(*(const PRL_GLOBAL typename T::Quad*)(p + i));
+    adam32_quad(c, gr, x, mq, vq);
+    *(PRL_GLOBAL f32x4_u*)(m + i) = mq;
+    *(PRL_GLOBAL f32x4_u*)(v + i) = vq;
+    if (MASTER) *(PRL_GLOBAL f32x4_u*)(w + i) = x;
+    *(PRL_GLOBAL typename T::Quad*)(p + i) = T::narrow(x);
+  } else if (i < left) {
+    adam32_part<T, MASTER>(c, p + i, g + i, MASTER ? w + i : w, m + i, v + i, left - i);
+  }
+}
+
+// STEP: the whole step; otherwise the norm alone
+template <bool STEP>
+__global__ __launch_bounds__(64 * L_SMALL_WAVES) void list_small_kernel(const SmallArgs a) {
+  __shared__ double s_part[L_SMALL_WAVES];
+  __shared__ Coef s_coef[L_SMALL];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const unsigned first = lane < a.count ? a.start[lane] : 0xffffffffu;   // of tensor `lane`
+  const auto entry = [&](int item) { return __popcll(__ballot(first <= (unsigned)item)) - 1; };
+  // the scalars beside the norm's loads, by the wave with the fewest blocks
+  if (STEP && wave == L_SMALL_WAVES - 1 && lane < a.count)
+    s_coef[lane] = next_coef(a.groups[a.kind[lane] >> 16], a.step[lane], 1.0f);
+  if (a.norm != nullptr) {
+    double acc = 0.0;
+    for (int b = wave; b < a.items; b += 4 * L_SMALL_WAVES) {
+      f32x4 f[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        f[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int item = b + L_SMALL_WAVES * u;
+        if (item < a.items) {
+          const int e = entry(item), i = (item - (int)a.start[e]) * PRL_LIST_BLOCK + 4 * lane, left = a.n[e] - i;
+          const unsigned dtype = a.kind[e] & 0xff;
+          if (dtype == PRL_LIST_F32) f[u] = load_quad<F32>(a.grad[e], i, left);
+          else if (dtype == PRL_LIST_BF16) f[u] = load_quad<BF16>(a.grad[e], i, left);
+          else f[u] = load_quad<F16>(a.grad[e], i, left);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc = fma((double)f[u][e], (double)f[u][e], acc);
+    }
+    acc = wave_sum_f64_to63(acc);
+    if (lane == 63) s_part[wave] = acc;
+  }
+  __syncthreads();
+  float clip = 1.0f;
+  if (a.norm != nullptr) {
+    double sum = 0.0;
+    for (int w = 0; w < L_SMALL_WAVES; ++w) sum += s_part[w];
+    const float norm = (float)sqrt(sum);
+    if (t == 0) a.norm[0] = norm;
+    clip = clip_coef(norm, a.max_norm);
+  }
+  if (!STEP) return;
+  for (int item = wave; item < a.items; item += L_SMALL_WAVES) {
+    const int e = entry(item), base = (item - (int)a.start[e]) * PRL_LIST_BLOCK;
+    Coef c = s_coef[e];
+    c.clip = clip;
+    const bool master = a.master[e] != nullptr;
+    const unsigned dtype = a.kind[e] & 0xff;
+    if (dtype == PRL_LIST_F32) small_item<F32, false>(c, a, e, base);
+    else if (dtype == PRL_LIST_BF16) {
+      if (master) small_item<BF16, true>(c, a, e, base);
+      else small_item<BF16, false>(c, a, e, base);
+    } else {
+      if (master) small_item<F16, true>(c, a, e, base);
+      else small_item<F16, false>(c, a, e, base);
+    }
+  }
+}
+
 // ---- host --------------------------------------------------------------------------------------
 inline int64_t list_total(const prl_list_entry* e, int64_t count) {
   int64_t total = 0;
@@ -549,7 +686,7 @@ int launch_norm(const prl_list_entry* e, int64_t count, bool once, double* parti
     a.x[a.count] = e[i].grad;
     a.n[a.count] = e[i].numel;
     a.start[a.count] = (unsigned)blocks;
-    a.dtype[a.count] = (unsigned char)e[i].dtype;
+    a.dtype[a.count] = (unsigned)e[i].dtype;
     ++a.count;
     blocks += cdiv(e[i].numel, a.chunk);
   }
@@ -647,16 +784,59 @@ int launch_adam8(const prl_list_entry* e, int64_t count, const Coef* coef, hipSt
   return PRL_OK;
 }
 
+// whether one launch of list_small_kernel takes the list
+bool is_small(const prl_list_entry* e, int64_t count, int64_t n_groups) {
+  if (count > L_SMALL || n_groups > L_GROUPS) return false;
+  int64_t items = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    items += cdiv(e[i].numel, PRL_LIST_BLOCK);
+    if (items > L_SMALL_ITEMS) return false;
+  }
+  return true;
+}
+
+template <bool STEP>
+int launch_small(const prl_list_entry* e, int64_t count, const prl_list_group* groups, int64_t n_groups,
+                 float max_norm, float* norm, hipStream_t st) {
+  SmallArgs a{};
+  int64_t items = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    a.start[i] = (unsigned)items;
+    items += cdiv(e[i].numel, PRL_LIST_BLOCK);
+    a.grad[i] = e[i].grad;
+    a.n[i] = (int)e[i].numel;
+    a.kind[i] = (unsigned)e[i].dtype;
+    if (!STEP) continue;
+    a.param[i] = e[i].param;
+    a.master[i] = e[i].master;
+    a.m[i] = e[i].exp_avg;
+    a.r[i] = e[i].second;
+    a.m_scale[i] = e[i].exp_avg_scale;
+    a.r_scale[i] = e[i].second_scale;
+    a.step[i] = e[i].step;
+    a.kind[i] |= (unsigned)e[i].bits << 8 | (unsigned)e[i].group << 16;
+  }
+  for (int64_t g = 0; g < n_groups; ++g) a.groups[g] = groups[g];
+  a.norm = norm;
+  a.max_norm = max_norm;
+  a.count = (int)count;
+  a.items = (int)items;
+  hipLaunchKernelGGL(list_small_kernel<STEP>, dim3(1), dim3(64 * L_SMALL_WAVES), 0, st, a);
+  PRL_LAUNCH_CHECK("list_small");
+  return PRL_OK;
+}
+
+constexpr int64_t L_MAX_COUNT = 1 << 24, L_MAX_NUMEL = (int64_t)1 << 40;
 // sizes and types; a list's total stays below 2^40 values, so every launch's grid fits
 int check_list(const char* what, const prl_list_entry* e, int64_t count) {
-  PRL_REQUIRE(count >= 0 && count < (1 << 24), "%s: %lld tensors", what, (long long)count);
+  PRL_REQUIRE(count >= 0 && count < L_MAX_COUNT, "%s: %lld tensors", what, (long long)count);
   PRL_REQUIRE(count == 0 || e != nullptr, "%s: null entries", what);
   int64_t total = 0;
   for (int64_t i = 0; i < count; ++i) {
-    PRL_REQUIRE(e[i].numel >= 0 && e[i].numel < (int64_t)1 << 40, "%s: tensor %lld: bad size %lld", what,
+    PRL_REQUIRE(e[i].numel >= 0 && e[i].numel < L_MAX_NUMEL, "%s: tensor %lld: bad size %lld", what,
                 (long long)i, (long long)e[i].numel);
     total += e[i].numel;
-    PRL_REQUIRE(total < (int64_t)1 << 40, "%s: list too large", what);
+    PRL_REQUIRE(total < L_MAX_NUMEL, "%s: list too large", what);
     PRL_REQUIRE(e[i].dtype >= PRL_LIST_F32 && e[i].dtype <= PRL_LIST_F16, "%s: tensor %lld: unknown type %d", what,
                 (long long)i, (int)e[i].dtype);
     PRL_REQUIRE(e[i].numel == 0 || e[i].grad, "%s: tensor %lld: null grad", what, (long long)i);
@@ -670,17 +850,21 @@ int check_list(const char* what, const prl_list_entry* e, int64_t count) {
 
 using namespace prl;
 
-extern "C" int64_t prl_list_workspace_bytes(int64_t count) {
-  if (count < 0) return -1;
+extern "C" int64_t prl_list_workspace_bytes(const prl_list_entry* entries, int64_t count, int64_t n_groups) {
+  if (count < 0 || count >= L_MAX_COUNT || (count > 0 && entries == nullptr)) return -1;
+  for (int64_t i = 0; i < count; ++i)
+    if (entries[i].numel < 0 || entries[i].numel >= L_MAX_NUMEL) return -1;
+  if (is_small(entries, count, n_groups)) return 0;
   return (int64_t)sizeof(Coef) * count + 8 * (L_NORM_BLOCKS + count);
 }
 
 extern "C" int prl_list_norm(const prl_list_entry* entries, int64_t count, float* norm, void* workspace,
                              int64_t workspace_bytes, void* stream) {
   if (int rc = check_list("prl_list_norm", entries, count)) return rc;
-  PRL_REQUIRE(norm && workspace, "prl_list_norm: null pointer");
-  PRL_REQUIRE(aligned16(workspace) && workspace_bytes >= prl_list_workspace_bytes(count),
-              "prl_list_norm: workspace too small or not 16-B aligned");
+  PRL_REQUIRE(norm, "prl_list_norm: null norm");
+  if (is_small(entries, count, 0)) return launch_small<false>(entries, count, nullptr, 0, 0.0f, norm, as_stream(stream));
+  PRL_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= prl_list_workspace_bytes(entries, count, 0),
+              "prl_list_norm: workspace null, too small or not 16-B aligned");
   Coef* coef = static_cast<Coef*>(workspace);
   double* partial = reinterpret_cast<double*>(coef + count);
   int64_t n_partial = 0;
@@ -693,10 +877,8 @@ extern "C" int prl_list_adamw(const prl_list_entry* entries, int64_t count, cons
                               int64_t workspace_bytes, void* stream) {
   if (int rc = check_list("prl_list_adamw", entries, count)) return rc;
   if (count == 0 && norm == nullptr) return PRL_OK;
-  PRL_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= prl_list_workspace_bytes(count),
-              "prl_list_adamw: workspace null, too small or not 16-B aligned");
   PRL_REQUIRE(norm == nullptr || max_norm >= 0.0f, "prl_list_adamw: max_norm %g", (double)max_norm);
-  PRL_REQUIRE(count == 0 || groups, "prl_list_adamw: null groups");
+  PRL_REQUIRE(n_groups >= 0 && (n_groups == 0 || groups), "prl_list_adamw: null groups");
   for (int64_t i = 0; i < count; ++i) {
     const prl_list_entry& e = entries[i];
     PRL_REQUIRE(e.bits == 32 || e.bits == 8, "prl_list_adamw: tensor %lld: moments in %d bits", (long long)i, (int)e.bits);
@@ -716,6 +898,9 @@ extern "C" int prl_list_adamw(const prl_list_entry* entries, int64_t count, cons
                 "prl_list_adamw: tensor %lld: a pointer not aligned to its type", (long long)i);
   }
   hipStream_t st = as_stream(stream);
+  if (is_small(entries, count, n_groups)) return launch_small<true>(entries, count, groups, n_groups, max_norm, norm, st);
+  PRL_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= prl_list_workspace_bytes(entries, count, n_groups),
+              "prl_list_adamw: workspace null, too small or not 16-B aligned");
   Coef* coef = static_cast<Coef*>(workspace);
   double* partial = reinterpret_cast<double*>(coef + count);
   int64_t n_partial = 0;

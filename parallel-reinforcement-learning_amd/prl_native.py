@@ -117,7 +117,7 @@ SIGNATURES = {
 }
 # include/prl_optim.h: the optimizer operators over lists of tensors
 OPTIM_SIGNATURES = {
-    "prl_list_workspace_bytes": [_I64],
+    "prl_list_workspace_bytes": [_P, _I64, _I64],
     "prl_list_norm": [_P, _I64, _P, _P, _I64, _P],
     "prl_list_adamw": [_P, _I64, _P, _I64, _F32, _P, _P, _I64, _P],
 }
@@ -824,36 +824,45 @@ def _list_call(device, call):
         return call(torch._C._cuda_getCurrentRawStream(device.index))
 
 
+def list_workspace_bytes(entries: array, n_groups: int = 0) -> int:
+    """Workspace of list_norm (n_groups 0) / list_adamw for a list of these sizes."""
+    return int(lib().prl_list_workspace_bytes(entries.buffer_info()[0],
+                                              len(entries) // LIST_ENTRY_WORDS, n_groups))
+
+
 def list_norm(entries: array, device: torch.device) -> torch.Tensor:
     """prl_list_norm over the entries' grads (an array("q") of prl_list_entry words): a new 0-dim
     f32 tensor.  Scratch is allocated per call, so a captured graph owns its own."""
-    count = len(entries) // LIST_ENTRY_WORDS
-    need = int(lib().prl_list_workspace_bytes(count))
+    need = list_workspace_bytes(entries)
 
     def call(stream):
         norm = torch.empty((), dtype=torch.float32, device=device)
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
-        _check(lib().prl_list_norm(entries.buffer_info()[0], count, norm.data_ptr(), ws.data_ptr(),
-                                   need, stream), "prl_list_norm")
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+        _check(lib().prl_list_norm(entries.buffer_info()[0], len(entries) // LIST_ENTRY_WORDS,
+                                   norm.data_ptr(), ws.data_ptr() if need > 0 else None, need, stream),
+               "prl_list_norm")
         return norm
     return _list_call(device, call)
 
 
-def list_adamw(entries: array, groups: array, device: torch.device, max_norm=None):
+def list_adamw(entries: array, groups: array, device: torch.device, max_norm=None, need=None):
     """prl_list_adamw: one AdamW step of every entry (array("q") of prl_list_entry words; groups:
-    array("d") / bytes of prl_list_group words).  With max_norm the gradients are clipped by their
-    global norm, which is returned (a new 0-dim f32 tensor); None otherwise."""
-    count = len(entries) // LIST_ENTRY_WORDS
-    need = int(lib().prl_list_workspace_bytes(count))
+    the bytes of prl_list_group as an array("q")).  With max_norm the gradients are clipped by their
+    global norm, which is returned (a new 0-dim f32 tensor); None otherwise.  need:
+    list_workspace_bytes of the list, where the caller keeps it."""
+    n_groups = len(groups) // LIST_GROUP_WORDS
+    if need is None:
+        need = list_workspace_bytes(entries, n_groups)
 
     def call(stream):
         norm = None if max_norm is None else torch.empty((), dtype=torch.float32, device=device)
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
-        _check(lib().prl_list_adamw(entries.buffer_info()[0], count, groups.buffer_info()[0],
-                                    len(groups) // LIST_GROUP_WORDS,
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+        _check(lib().prl_list_adamw(entries.buffer_info()[0], len(entries) // LIST_ENTRY_WORDS,
+                                    groups.buffer_info()[0], n_groups,
                                     0.0 if max_norm is None else max_norm,
-                                    None if norm is None else norm.data_ptr(), ws.data_ptr(), need,
-                                    stream), "prl_list_adamw")
+                                    None if norm is None else norm.data_ptr(),
+                                    ws.data_ptr() if need > 0 else None, need, stream),
+               "prl_list_adamw")
         return norm
     return _list_call(device, call)
 

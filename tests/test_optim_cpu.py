@@ -30,7 +30,7 @@ def _adamw(entries, groups=((1e-3, 0.9, 0.999, 1e-8, 0.0, 0),), n_groups=None, w
     table = array("q", [w for e in entries for w in e])
     g = b"".join(struct.pack("5dq", *x) for x in groups)
     rc = L.prl_list_adamw(table.buffer_info()[0] if entries else None, len(entries), g, len(groups) if n_groups is None else n_groups,
-                          max_norm, norm, ws, L.prl_list_workspace_bytes(len(entries)) if bytes_ is None else bytes_, None)
+                          max_norm, norm, ws, 1 << 20 if bytes_ is None else bytes_, None)
     return rc, L.prl_last_error().decode()
 
 
@@ -49,15 +49,22 @@ def test_c_entry_refuses_bad_lists():
     for e, text in cases:
         rc, msg = _adamw([list_entry(**ok), list_entry(**e)])
         assert rc == -1 and text in msg, (e, msg)
-    assert _adamw([list_entry(**ok)], bytes_=64)[0] == -1
-    assert _adamw([list_entry(**ok)], ws=None)[0] == -1
-    assert _adamw([list_entry(**ok)], ws=(1 << 20) + 8)[0] == -1
+    long = [list_entry(**ok)] * 33          # more than the launch of a short list takes: a workspace is needed
+    assert _adamw(long, bytes_=64)[0] == -1
+    assert _adamw(long, ws=None)[0] == -1
+    assert _adamw(long, ws=(1 << 20) + 8)[0] == -1
     assert _adamw([list_entry(**ok)], norm=4096, max_norm=-1.0)[0] == -1
     assert _adamw([list_entry(**ok)], norm=4096, max_norm=float("nan"))[0] == -1
     assert _adamw([])[0] == 0          # nothing to do, nothing launched
     import prl_native
     L = prl_native.lib()
-    assert L.prl_list_workspace_bytes(-1) == -1
+    assert L.prl_list_workspace_bytes(None, -1, 1) == -1
+    def need(entries, groups=1):
+        t = array("q", [w for e in entries for w in e])
+        return L.prl_list_workspace_bytes(t.buffer_info()[0], len(entries), groups)
+    assert need([list_entry(**ok)] * 32) == 0 and need(long) >= 33 * 56
+    assert need([list_entry(**dict(ok, numel=160 * 256))]) == 0 and need([list_entry(**dict(ok, numel=160 * 256 + 1))]) > 0
+    assert need([list_entry(**ok)], 17) > 0 and need([list_entry(**dict(ok, numel=-1))]) == -1
     assert L.prl_list_norm(None, 1, 4096, 4096, 1 << 20, None) == -1
     assert L.prl_list_norm(None, -1, 4096, 4096, 1 << 20, None) == -1
     assert L.prl_list_norm(None, 0, None, 4096, 1 << 20, None) == -1

@@ -505,6 +505,74 @@ def test_learn_wide_policy_and_rnd_with_8_bit_moments():
     assert all(bool(torch.isfinite(p).all()) and not torch.equal(p, o) for p, o in zip(new, old))
 
 
+def test_step_runs_torch_hooks_and_shows_in_the_profiler():
+    from torch.optim.optimizer import register_optimizer_step_post_hook, register_optimizer_step_pre_hook
+    p = torch.nn.Parameter(torch.ones(10, device="cuda"))
+    p.grad = torch.ones_like(p)
+    opt = _optim().AdamW([p])
+    seen = []
+    hooks = [opt.register_step_pre_hook(lambda o, a, k: seen.append("pre")),
+             opt.register_step_post_hook(lambda o, a, k: seen.append("post")),
+             register_optimizer_step_pre_hook(lambda o, a, k: seen.append("global pre")),
+             register_optimizer_step_post_hook(lambda o, a, k: seen.append("global post"))]
+    for h in hooks:
+        opt.step(max_norm=1.0)
+        h.remove()
+    assert seen.count("pre") == 1 and seen.count("post") == 2
+    assert seen.count("global pre") == 3 and seen.count("global post") == 4
+    opt.step()
+    assert len(seen) == 10 and float(opt.state[p]["step"]) == 5.0
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        opt.step()
+    assert any("Optimizer.step#AdamW" in e.key for e in prof.key_averages())
+    before = p.detach().clone()
+    loss = opt.step(lambda: (p * 2.0).sum().backward() or torch.tensor(3.0))
+    assert float(loss) == 3.0 and not torch.equal(p.detach(), before)
+    sched = torch.optim.lr_scheduler.StepLR(opt, 1, gamma=0.5)
+    opt.step()
+    sched.step()
+    assert opt.param_groups[0]["lr"] == 0.5e-3
+
+
+def test_short_and_long_lists_agree():
+    """A list at the one-launch form's bounds (160 blocks of 256 values, 32 tensors, 16 groups) and past
+    each of them: the same step, up to the norm's summation order (off by one float32 rounding)."""
+    O = _optim()
+    sizes = [1024] * 39 + [1024 - 3]
+    for bits in (32, 8):
+        base, bgrads = _make([160 * 256], torch.float32, 4, lead=3)
+        over, ograds = _make([160 * 256, 1], torch.float32, 4, lead=3)
+        with torch.no_grad():
+            over[0].copy_(base[0])
+            ograds[0].copy_(bgrads[0])
+            ograds[1].zero_()
+        a, b = O.AdamW(base, state_bits=bits), O.AdamW(over, state_bits=bits)
+        for _ in range(2):
+            a.step()
+            b.step()
+        assert torch.equal(base[0], over[0])
+        a.step(max_norm=1.0)
+        b.step(max_norm=1.0)
+        n = R.norm64(bgrads)
+        assert abs(float(a.total_norm) - n) <= 1.01 * R.U32 * n and abs(float(b.total_norm) - n) <= 1.01 * R.U32 * n
+        # 33 tensors / 17 groups of the same values
+        runs = []
+        for split in (lambda ps: [dict(params=ps[:33])], lambda ps: [dict(params=ps[:32]), dict(params=ps[32:33])],
+                      lambda ps: [dict(params=[p]) for p in ps[:17]] + [dict(params=ps[17:33])]):
+            params, _ = _make(sizes, torch.float32, 4, lead=3)
+            opt = O.AdamW(split(params), state_bits=bits)
+            opt.step()
+            opt.step()
+            runs.append([p.detach().clone() for p in params[:33]])
+        few, _ = _make(sizes, torch.float32, 4, lead=3)
+        opt = O.AdamW(few[:32], state_bits=bits)
+        opt.step()
+        opt.step()
+        for r in runs:
+            assert all(torch.equal(x, y) for x, y in zip(r, runs[0]))
+            assert all(torch.equal(x, y.detach()) for x, y in zip(r, few[:32]))
+
+
 def test_refusals_on_the_device():
     O = _optim()
     p = torch.nn.Parameter(torch.ones(10, device="cuda"))
