@@ -39,14 +39,14 @@ _GLOBAL_HOOKS = [getattr(import_module("torch.optim.optimizer"), f"_global_optim
 def _dense(tensors, device, name):
     """The tensors, contiguous (those that are not: copies), after checking that they are dense
     device tensors of a known type on one device."""
-    if not all(map(is_, map(_layout, tensors), repeat(torch.strided))) or any(d != device for d in map(_device, tensors)):
+    if (set(map(_layout, tensors)) != {torch.strided} or set(map(_device, tensors)) != {device} or device < 0
+            or not _DTYPES.keys() >= set(map(_dtype, tensors))):
         for t in tensors:
             if t.layout is not torch.strided or not t.is_cuda:
                 raise ValueError(f"{name} must be a dense device tensor (got {t.layout} on {t.device})")
+            if t.dtype not in _DTYPES:
+                raise ValueError(f"{name} must be float32, bfloat16 or float16 (got {t.dtype})")
         raise ValueError(f"{name}: all must be on one device (got {sorted({str(t.device) for t in tensors})})")
-    for t in tensors:
-        if t.dtype not in _DTYPES:
-            raise ValueError(f"{name} must be float32, bfloat16 or float16 (got {t.dtype})")
     return tensors if all(map(_contiguous, tensors)) else [t.detach().contiguous() for t in tensors]
 
 
@@ -57,7 +57,7 @@ def grad_norm(tensors) -> torch.Tensor:
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not tensors:
         raise ValueError("grad_norm needs at least one tensor")
-    tensors = _dense(tensors, max(tensors[0].get_device(), 0), "a tensor of the list")
+    tensors = _dense(tensors, tensors[0].get_device(), "a tensor of the list")
     table = array("q", bytes(8 * _WORDS * len(tensors)))
     table[1::_WORDS] = array("q", map(_ptr, tensors))
     table[8::_WORDS] = array("q", map(_numel, tensors))
@@ -255,7 +255,7 @@ class _Plan:
         if not chosen:
             return
         self.device = self.params[0].device
-        _dense(self.params, max(self.params[0].get_device(), 0), "a parameter")
+        _dense(self.params, self.params[0].get_device(), "a parameter")
         columns = []
         for p, g, _, group in chosen:
             if not p.is_contiguous():
@@ -294,9 +294,8 @@ class _Plan:
             return False
         values = list(chain.from_iterable(map(dict.values, state.values())))
         return (len(values) == len(self.values) and all(map(is_, values, self.values))
-                and list(map(_numel, self.params)) == self.numels
-                and list(map(_dtype, self.params)) == self.dtypes and all(map(_contiguous, self.params))
-                and list(map(_ptr, self.tensors)) == self.at)
+                and list(map(_numel, self.params)) == self.numels and all(map(_contiguous, self.params))
+                and list(map(_ptr, self.tensors)) == self.at)     # (the types: by the gradients, in fill())
 
     def fill(self, grads):
         """The table with the gradients' addresses, and the tensors that these are of."""

@@ -27,10 +27,16 @@ typedef unsigned u32_u __attribute__((aligned(1)));
 #define PRL_GLOBAL __attribute__((address_space(1)))
 
 constexpr int L_THREADS = 256;
-constexpr int L_BATCH = 64;           // tensors per launch of the norm and the 32-bit step
-constexpr int L_BATCH8 = 48;          // of the 8-bit step (more pointers each; arguments stay under 4 KB)
-constexpr int L_BATCH_BEGIN = 192;    // of list_begin_kernel
+constexpr int L_BATCH_NORM = 128;     // tensors per launch of the norm,
+constexpr int L_BATCH = 64;           // of the 32-bit step,
+constexpr int L_BATCH8 = 48;          // of the 8-bit step (more pointers each),
+constexpr int L_BATCH_BEGIN = 256;    // of list_begin_kernel: as many as 4 KB of arguments hold
 constexpr int L_GROUPS = 16;
+// Values per workgroup of a step.  32 bits: 2,048 (50 M bfloat16 values with masters 255 us; 4,096: 260,
+// 8,192: 266).  8 bits: 2,048 of float32 weights or masters (126 M values 336 us; 1,024: 351, 4,096: 350),
+// 4,096 of 16-bit weights alone, where the instructions count and with them what a workgroup
+// does once (126 M values 286 us; 1,024: 352, 2,048: 302).
+constexpr int L_CHUNK32 = 2048, L_CHUNK8 = 2048, L_CHUNK8_16 = 4096;
 constexpr int L_COEF = 12;            // floats per tensor in the workspace
 constexpr int L_NORM_BLOCKS = 2048;   // partial sums of a norm, besides one per tensor
 
@@ -91,10 +97,10 @@ typedef Half<_Float16> F16;
 
 // ---- norm ------------------------------------------------------------------------------------
 struct NormArgs {
-  const void* x[L_BATCH];
-  int64_t n[L_BATCH];
-  unsigned start[L_BATCH];
-  unsigned dtype[L_BATCH];
+  const void* x[L_BATCH_NORM];
+  int64_t n[L_BATCH_NORM];
+  unsigned start[L_BATCH_NORM];
+  unsigned dtype[L_BATCH_NORM];
   int64_t chunk;
   int count;
 };
@@ -250,7 +256,6 @@ struct Adam32Args {
   unsigned start[L_BATCH];
   unsigned which[L_BATCH];   // the tensor's place in the call (its Coef), dtype in the top bits
   const Coef* coef;
-  int64_t chunk;
   int count;
 };
 static_assert(sizeof(Adam32Args) <= 4096, "kernel arguments");
@@ -334,8 +339,8 @@ __device__ inline void adam32_chunk(const Coef& c, void* pp, const void* pg, flo
 
 __global__ __launch_bounds__(L_THREADS) void list_adam32_kernel(const Adam32Args a) {
   const int e = find_entry(a.start, a.count, blockIdx.x);
-  const int64_t n = a.n[e], lo = (int64_t)(blockIdx.x - a.start[e]) * a.chunk;
-  const int64_t hi = lo + a.chunk < n ? lo + a.chunk : n;
+  const int64_t n = a.n[e], lo = (int64_t)(blockIdx.x - a.start[e]) * L_CHUNK32;
+  const int64_t hi = lo + L_CHUNK32 < n ? lo + L_CHUNK32 : n;
   const unsigned which = a.which[e], dtype = which >> 30;
   const Coef c = a.coef[which & 0x3fffffffu];
   void* p = a.param[e];
@@ -366,7 +371,6 @@ struct Adam8Args {
   unsigned start[L_BATCH8];
   unsigned which[L_BATCH8];
   const Coef* coef;
-  int64_t chunk;
   int count;
 };
 static_assert(sizeof(Adam8Args) <= 4096, "kernel arguments");
@@ -391,6 +395,29 @@ __device__ inline unsigned draw_bits(unsigned at, unsigned seed) {
   h = (h ^ (h >> 15)) * 0x846CA68Bu;
   asm("" : "+v"(h));   // opaque: the compiler would form h << 16 by a third multiplication (quarter rate)
   return h;
+}
+
+// the largest of the four magnitudes, as bits (a NaN is larger than an infinity)
+__device__ inline unsigned max_bits(const float (&x)[4]) {
+  unsigned most = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const unsigned b = __float_as_uint(x[e]) & 0x7fffffffu;
+    most = most > b ? most : b;
+  }
+  return most;
+}
+
+// The root of v >= 0 by one step of Newton's method on v_rsq_f32, half the instructions of sqrtf():
+// within 2^-44 of the root before its last rounding.  Below 2^-126 it comes out small (a positive v
+// still gives a positive root), and an infinite v gives NaN: a block is taken again with sqrtf() unless its
+// largest root lies from 2^-40 to the largest finite number.  In such a block a root below 2^-63 is the
+// smallest code, right or small, and adds nothing to an eps of 2^-40 or more in the denominator.
+constexpr unsigned QUICK_FROM = 0x2b800000u;   // 2^-40
+__device__ inline float quick_root(float v) {
+  const float y = __builtin_amdgcn_rsqf(fmaxf(v, 0x1p-126f));
+  const float s = v * y;
+  return fmaf(fmaf(-s, s, v), 0.5f * y, s);
 }
 
 // 256 / A for a block's largest magnitude A given as its bits; 0: the block is held as zeros
@@ -435,16 +462,26 @@ __device__ inline void adam8_block(const Coef& c, PRL_GLOBAL typename T::One* p,
                 __builtin_amdgcn_cvt_f32_fp8(mq, 2), __builtin_amdgcn_cvt_f32_fp8(mq, 3)};
   float r[4] = {__builtin_amdgcn_cvt_f32_fp8(rq, 0), __builtin_amdgcn_cvt_f32_fp8(rq, 1),
                 __builtin_amdgcn_cvt_f32_fp8(rq, 2), __builtin_amdgcn_cvt_f32_fp8(rq, 3)};
+  float v[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     m[e] = m[e] * ma;
     r[e] = r[e] * ra;
-    float v = r[e] * r[e];
-    adam_moments(c, gr[e], m[e], v);
-    r[e] = sqrtf(v);
-    x[e] = adam_weight(c, x[e], m[e], r[e]);
-    if (!WHOLE && e >= left) m[e] = r[e] = 0.0f;   // past the tensor's end nothing counts (a NaN clip would)
+    v[e] = r[e] * r[e];
+    adam_moments(c, gr[e], m[e], v[e]);
+    if (!WHOLE && e >= left) m[e] = v[e] = 0.0f;   // past the tensor's end nothing counts (a NaN clip would)
+    r[e] = quick_root(v[e]);
   }
+  const unsigned m_max = wave_max_u32(max_bits(m));
+  unsigned r_max = wave_max_u32(max_bits(r));
+  // not the quick root's range (see there), or an eps that its error far below r_max could reach
+  if (r_max - QUICK_FROM >= 0x7f800000u - QUICK_FROM || c.eps < 0x1p-40f) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = sqrtf(v[e]);
+    r_max = wave_max_u32(max_bits(r));
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = adam_weight(c, x[e], m[e], r[e]);
   if (left >= 4) {
     if (MASTER) PRL_STORE_NT(f32x4_u, w + i, x);
     PRL_STORE_NT(Quad, p + i, T::narrow(x));
@@ -452,15 +489,6 @@ __device__ inline void adam8_block(const Coef& c, PRL_GLOBAL typename T::One* p,
     if (MASTER) store_part<F32>(w + i, left, x);
     store_part<T>(p + i, left, x);
   }
-  unsigned m_max = 0, r_max = 0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const unsigned mb = __float_as_uint(m[e]) & 0x7fffffffu, rb = __float_as_uint(r[e]);   // r >= 0 or NaN
-    m_max = m_max > mb ? m_max : mb;
-    r_max = r_max > rb ? r_max : rb;
-  }
-  m_max = wave_max_u32(m_max);
-  r_max = wave_max_u32(r_max);
   // both factors in one division: the first moment's in lane 0, the second's in lane 1
   const float k = block_factor(lane & 1 ? r_max : m_max);
   const float km = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(k), 0));
@@ -503,6 +531,9 @@ __device__ inline void adam8_block(const Coef& c, PRL_GLOBAL typename T::One* p,
   }
 }
 
+__host__ __device__ inline int adam8_chunk_of(unsigned dtype, bool master) {
+  return dtype == PRL_LIST_F32 || master ? L_CHUNK8 : L_CHUNK8_16;
+}
 template <typename T, bool MASTER>
 __device__ inline void adam8_chunk(const Coef& c, const Adam8Args& a, int e, int64_t lo, int64_t hi, int64_t n) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -521,9 +552,10 @@ __device__ inline void adam8_chunk(const Coef& c, const Adam8Args& a, int e, int
 
 __global__ __launch_bounds__(L_THREADS) void list_adam8_kernel(const Adam8Args a) {
   const int e = find_entry(a.start, a.count, blockIdx.x);
-  const int64_t n = a.n[e], lo = (int64_t)(blockIdx.x - a.start[e]) * a.chunk;
-  const int64_t hi = lo + a.chunk < n ? lo + a.chunk : n;
   const unsigned which = a.which[e], dtype = which >> 30;
+  const int chunk = adam8_chunk_of(dtype, a.master[e] != nullptr);
+  const int64_t n = a.n[e], lo = (int64_t)(blockIdx.x - a.start[e]) * chunk;
+  const int64_t hi = lo + chunk < n ? lo + chunk : n;
   const Coef c = a.coef[which & 0x3fffffffu];
   const bool master = a.master[e] != nullptr;
   if (dtype == PRL_LIST_F32) adam8_chunk<F32, false>(c, a, e, lo, hi, n);
@@ -674,7 +706,7 @@ int launch_norm(const prl_list_entry* e, int64_t count, bool once, double* parti
   a.chunk = tile * (1 + list_total(e, count) / (tile * L_NORM_BLOCKS));
   int64_t done = 0, blocks = 0;
   for (int64_t i = 0; i <= count; ++i) {
-    if (a.count == L_BATCH || (i == count && a.count > 0)) {
+    if (a.count == L_BATCH_NORM || (i == count && a.count > 0)) {
       if (once) hipLaunchKernelGGL(list_norm_kernel<true>, dim3((unsigned)blocks), dim3(L_THREADS), 0, st, a, partial + done);
       else hipLaunchKernelGGL(list_norm_kernel<false>, dim3((unsigned)blocks), dim3(L_THREADS), 0, st, a, partial + done);
       PRL_LAUNCH_CHECK("list_norm");
@@ -731,7 +763,6 @@ int launch_begin(const prl_list_entry* e, int64_t count, const prl_list_group* g
 int launch_adam32(const prl_list_entry* e, int64_t count, const Coef* coef, hipStream_t st) {
   Adam32Args a{};
   a.coef = coef;
-  a.chunk = 4 * L_THREADS * 4;
   int64_t blocks = 0;
   for (int64_t i = 0; i <= count; ++i) {
     if (a.count == L_BATCH || (i == count && a.count > 0)) {
@@ -750,7 +781,7 @@ int launch_adam32(const prl_list_entry* e, int64_t count, const Coef* coef, hipS
     a.n[k] = e[i].numel;
     a.start[k] = (unsigned)blocks;
     a.which[k] = (unsigned)i | (unsigned)e[i].dtype << 30;
-    blocks += cdiv(e[i].numel, a.chunk);
+    blocks += cdiv(e[i].numel, L_CHUNK32);
   }
   return PRL_OK;
 }
@@ -758,7 +789,6 @@ int launch_adam32(const prl_list_entry* e, int64_t count, const Coef* coef, hipS
 int launch_adam8(const prl_list_entry* e, int64_t count, const Coef* coef, hipStream_t st) {
   Adam8Args a{};
   a.coef = coef;
-  a.chunk = 4 * L_THREADS * 4;
   int64_t blocks = 0;
   for (int64_t i = 0; i <= count; ++i) {
     if (a.count == L_BATCH8 || (i == count && a.count > 0)) {
@@ -779,7 +809,7 @@ int launch_adam8(const prl_list_entry* e, int64_t count, const Coef* coef, hipSt
     a.n[k] = e[i].numel;
     a.start[k] = (unsigned)blocks;
     a.which[k] = (unsigned)i | (unsigned)e[i].dtype << 30;
-    blocks += cdiv(e[i].numel, a.chunk);
+    blocks += cdiv(e[i].numel, adam8_chunk_of((unsigned)e[i].dtype, e[i].master != nullptr));
   }
   return PRL_OK;
 }
