@@ -84,7 +84,10 @@ struct Half {   // __bf16 / _Float16: conversions round to nearest even
   typedef u16x4_u Quad;
   typedef unsigned short One;
   static __device__ inline float widen1(unsigned short x) { return (float)__builtin_bit_cast(H, x); }
-  static __device__ inline unsigned short narrow1(float x) { return __builtin_bit_cast(unsigned short, (H)x); }
+  static __device__ inline unsigned short narrow1(float x) {
+    asm("" : "+v"(x));   // of the float32 value: a float16 one would be formed with the sum before it (v_fma_mix)
+    return __builtin_bit_cast(unsigned short, (H)x);
+  }
   static __device__ inline f32x4 widen(u16x4 q) {
     return f32x4{widen1(q.x), widen1(q.y), widen1(q.z), widen1(q.w)};
   }
@@ -261,8 +264,9 @@ struct Adam32Args {
 static_assert(sizeof(Adam32Args) <= 4096, "kernel arguments");
 
 __device__ inline float adam_weight(const Coef& c, float w, float m, float rms) {
-  return w * c.decay - c.step_size * (m * __builtin_amdgcn_rcpf(rms * c.inv_bc2_sqrt + c.eps));
+  return fmaf(-c.step_size, m * __builtin_amdgcn_rcpf(fmaf(rms, c.inv_bc2_sqrt, c.eps)), w * c.decay);
 }
+// one rounding per operation, as written: the 8-bit moments' codes follow from these bits
 __device__ inline void adam_moments(const Coef& c, float g, float& m, float& v) {
   g = g * c.clip;
   m = m + (g - m) * c.omb1;
@@ -375,16 +379,19 @@ struct Adam8Args {
 };
 static_assert(sizeof(Adam8Args) <= 4096, "kernel arguments");
 
-// the largest of an unsigned over the wave, in every lane (as wave_sum_f32_to63, then lane 63's)
-__device__ inline unsigned wave_max_u32(unsigned x) {
-  const auto step = [](unsigned v, int moved) { return v > (unsigned)moved ? v : (unsigned)moved; };
-  x = step(x, __builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, false));
-  x = step(x, __builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, false));
-  x = step(x, __builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xF, 0xF, false));
-  x = step(x, __builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xF, 0xF, false));
-  x = step(x, __builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false));
-  x = step(x, __builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false));
-  return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
+// the largest of x and of y over the wave: one swap of halves (x's in lanes 0 - 31, y's in 32 - 63), then
+// five DPP steps for both (xor 1, xor 2, half-row mirror, row mirror, row 0 / 2's lane 15 broadcast)
+__device__ inline void wave_max_pair(unsigned& x, unsigned& y) {
+  const auto moved = [](unsigned v, int m) { return v > (unsigned)m ? v : (unsigned)m; };
+  const auto s = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+  unsigned v = s[0] > s[1] ? s[0] : s[1];
+  v = moved(v, __builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));
+  v = moved(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));
+  v = moved(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, false));
+  v = moved(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, false));
+  v = moved(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false));
+  x = (unsigned)__builtin_amdgcn_readlane((int)v, 31);
+  y = (unsigned)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // a value's two 16-bit draws at this step are the halves of h ^ (h >> 16), h = draw_bits(its index
@@ -397,12 +404,14 @@ __device__ inline unsigned draw_bits(unsigned at, unsigned seed) {
   return h;
 }
 
-// the largest of the four magnitudes, as bits (a NaN is larger than an infinity)
+// the largest of the four magnitudes, as bits (a NaN is larger than an infinity); the roots are
+// positive, or a NaN of either sign: larger than an infinity too
+template <bool SIGNED>
 __device__ inline unsigned max_bits(const float (&x)[4]) {
   unsigned most = 0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const unsigned b = __float_as_uint(x[e]) & 0x7fffffffu;
+    const unsigned b = __float_as_uint(x[e]) & (SIGNED ? 0x7fffffffu : 0xffffffffu);
     most = most > b ? most : b;
   }
   return most;
@@ -458,10 +467,9 @@ __device__ inline void adam8_block(const Coef& c, PRL_GLOBAL typename T::One* p,
       }
   }
   const float ma = ms[0] * 0x1p-8f, ra = rs[0] * 0x1p-8f;
-  float m[4] = {__builtin_amdgcn_cvt_f32_fp8(mq, 0), __builtin_amdgcn_cvt_f32_fp8(mq, 1),
-                __builtin_amdgcn_cvt_f32_fp8(mq, 2), __builtin_amdgcn_cvt_f32_fp8(mq, 3)};
-  float r[4] = {__builtin_amdgcn_cvt_f32_fp8(rq, 0), __builtin_amdgcn_cvt_f32_fp8(rq, 1),
-                __builtin_amdgcn_cvt_f32_fp8(rq, 2), __builtin_amdgcn_cvt_f32_fp8(rq, 3)};
+  const auto m01 = __builtin_amdgcn_cvt_pk_f32_fp8(mq, false), m23 = __builtin_amdgcn_cvt_pk_f32_fp8(mq, true);
+  const auto r01 = __builtin_amdgcn_cvt_pk_f32_fp8(rq, false), r23 = __builtin_amdgcn_cvt_pk_f32_fp8(rq, true);
+  float m[4] = {m01[0], m01[1], m23[0], m23[1]}, r[4] = {r01[0], r01[1], r23[0], r23[1]};
   float v[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -472,13 +480,15 @@ __device__ inline void adam8_block(const Coef& c, PRL_GLOBAL typename T::One* p,
     if (!WHOLE && e >= left) m[e] = v[e] = 0.0f;   // past the tensor's end nothing counts (a NaN clip would)
     r[e] = quick_root(v[e]);
   }
-  const unsigned m_max = wave_max_u32(max_bits(m));
-  unsigned r_max = wave_max_u32(max_bits(r));
+  unsigned m_max = max_bits<true>(m), r_max = max_bits<false>(r);
+  wave_max_pair(m_max, r_max);
   // not the quick root's range (see there), or an eps that its error far below r_max could reach
   if (r_max - QUICK_FROM >= 0x7f800000u - QUICK_FROM || c.eps < 0x1p-40f) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) r[e] = sqrtf(v[e]);
-    r_max = wave_max_u32(max_bits(r));
+    unsigned again = m_max;
+    r_max = max_bits<false>(r);
+    wave_max_pair(again, r_max);
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) x[e] = adam_weight(c, x[e], m[e], r[e]);
@@ -494,13 +504,14 @@ __device__ inline void adam8_block(const Coef& c, PRL_GLOBAL typename T::One* p,
   const float km = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(k), 0));
   const float kr = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(k), 1));
   // stochastic rounding to e4m3: the conversion adds its random bits below the mantissa bits it keeps
-  // and truncates, the sign aside; 16 of the 20 are drawn, the rest are 0
+  // and truncates, the sign aside; 16 of the 20 are drawn, the rest are 0.  (A * k may come out an ulp
+  // above 256: no draw carries that over 16 ulps to the next code.)
   unsigned d[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) d[e] = draw_bits(at + i + e, c.seed);
   int mw = 0, rw = 0;
   if (km > 0.0f) {
-    const auto y = [&](int e) { return __builtin_amdgcn_fmed3f(m[e] * km, -256.0f, 256.0f); };
+    const auto y = [&](int e) { return m[e] * km; };
     const auto draw = [&](int e) { return (d[e] << 16) ^ (d[e] & 0xffff0000u); };
     mw = __builtin_amdgcn_cvt_sr_fp8_f32(y(0), draw(0), mw, 0);
     mw = __builtin_amdgcn_cvt_sr_fp8_f32(y(1), draw(1), mw, 1);
@@ -508,7 +519,7 @@ __device__ inline void adam8_block(const Coef& c, PRL_GLOBAL typename T::One* p,
     mw = __builtin_amdgcn_cvt_sr_fp8_f32(y(3), draw(3), mw, 3);
   }
   if (kr > 0.0f) {   // an r above 0 stays above 0: 2^-9 is the smallest code
-    const auto y = [&](int e) { return r[e] > 0.0f ? __builtin_amdgcn_fmed3f(r[e] * kr, 0x1p-9f, 256.0f) : 0.0f; };
+    const auto y = [&](int e) { return r[e] > 0.0f ? fmaxf(r[e] * kr, 0x1p-9f) : 0.0f; };
     const auto draw = [&](int e) { return d[e] & 0xffff0000u; };
     rw = __builtin_amdgcn_cvt_sr_fp8_f32(y(0), draw(0), rw, 0);
     rw = __builtin_amdgcn_cvt_sr_fp8_f32(y(1), draw(1), rw, 1);

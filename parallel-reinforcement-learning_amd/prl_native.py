@@ -815,15 +815,6 @@ def list_entry(param=0, grad=0, master=0, exp_avg=0, second=0, exp_avg_scale=0, 
             dtype | bits << 32, group)
 
 
-def _list_call(device, call):
-    """call(stream) with `device` current and its current stream (a list's tensors may live on
-    another device than the current one)."""
-    if device.index == torch.cuda.current_device():
-        return call(torch._C._cuda_getCurrentRawStream(device.index))
-    with torch.cuda.device(device):
-        return call(torch._C._cuda_getCurrentRawStream(device.index))
-
-
 def list_workspace_bytes(entries: array, n_groups: int = 0) -> int:
     """Workspace of list_norm (n_groups 0) / list_adamw for a list of these sizes."""
     return int(lib().prl_list_workspace_bytes(entries.buffer_info()[0],
@@ -831,40 +822,41 @@ def list_workspace_bytes(entries: array, n_groups: int = 0) -> int:
 
 
 def list_norm(entries: array, device: torch.device) -> torch.Tensor:
-    """prl_list_norm over the entries' grads (an array("q") of prl_list_entry words): a new 0-dim
-    f32 tensor.  Scratch is allocated per call, so a captured graph owns its own."""
+    """prl_list_norm over the entries' grads (an array("q") of prl_list_entry words) on device's
+    current stream: a new 0-dim f32 tensor.  Scratch is allocated per call, so a captured graph owns
+    its own."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return list_norm(entries, device)
     need = list_workspace_bytes(entries)
-
-    def call(stream):
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
-        _check(lib().prl_list_norm(entries.buffer_info()[0], len(entries) // LIST_ENTRY_WORDS,
-                                   norm.data_ptr(), ws.data_ptr() if need > 0 else None, need, stream),
-               "prl_list_norm")
-        return norm
-    return _list_call(device, call)
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+    _check(lib().prl_list_norm(entries.buffer_info()[0], len(entries) // LIST_ENTRY_WORDS,
+                               norm.data_ptr(), None if ws is None else ws.data_ptr(), need,
+                               torch._C._cuda_getCurrentRawStream(device.index)), "prl_list_norm")
+    return norm
 
 
 def list_adamw(entries: array, groups: array, device: torch.device, max_norm=None, need=None):
-    """prl_list_adamw: one AdamW step of every entry (array("q") of prl_list_entry words; groups:
-    the bytes of prl_list_group as an array("q")).  With max_norm the gradients are clipped by their
-    global norm, which is returned (a new 0-dim f32 tensor); None otherwise.  need:
-    list_workspace_bytes of the list, where the caller keeps it."""
+    """prl_list_adamw on device's current stream: one AdamW step of every entry (array("q") of
+    prl_list_entry words; groups: the bytes of prl_list_group as an array("q")).  With max_norm the
+    gradients are clipped by their global norm, which is returned (a new 0-dim f32 tensor); None
+    otherwise.  need: list_workspace_bytes of the list, where the caller keeps it."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return list_adamw(entries, groups, device, max_norm, need)
     n_groups = len(groups) // LIST_GROUP_WORDS
     if need is None:
         need = list_workspace_bytes(entries, n_groups)
-
-    def call(stream):
-        norm = None if max_norm is None else torch.empty((), dtype=torch.float32, device=device)
-        ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
-        _check(lib().prl_list_adamw(entries.buffer_info()[0], len(entries) // LIST_ENTRY_WORDS,
-                                    groups.buffer_info()[0], n_groups,
-                                    0.0 if max_norm is None else max_norm,
-                                    None if norm is None else norm.data_ptr(),
-                                    ws.data_ptr() if need > 0 else None, need, stream),
-               "prl_list_adamw")
-        return norm
-    return _list_call(device, call)
+    norm = None if max_norm is None else torch.empty((), dtype=torch.float32, device=device)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+    _check(lib().prl_list_adamw(entries.buffer_info()[0], len(entries) // LIST_ENTRY_WORDS,
+                                groups.buffer_info()[0], n_groups,
+                                0.0 if max_norm is None else max_norm,
+                                None if norm is None else norm.data_ptr(),
+                                None if ws is None else ws.data_ptr(), need,
+                                torch._C._cuda_getCurrentRawStream(device.index)), "prl_list_adamw")
+    return norm
 
 
 def ppo_update_last_plan() -> dict:
