@@ -160,7 +160,10 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """torch's, except that the state keeps its own types (torch casts every state tensor to the
-        parameter's) and that this optimizer's state_bits / master stay."""
+        parameter's), and that this optimizer's state_bits / master stay: state of the other form
+        is refused by the next step."""
+        if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
+            raise ValueError("the state is of an AdamW with amsgrad or maximize")
         own = [(g["state_bits"], g["master"]) for g in self.param_groups]
         super().load_state_dict(state_dict)
         for g, (bits, master) in zip(self.param_groups, own):
@@ -172,7 +175,8 @@ class AdamW(torch.optim.Optimizer):
                 if k == "step":
                     v = torch.as_tensor(v, dtype=torch.float32).reshape(())
                 if torch.is_tensor(v):
-                    self.state[p][k] = v.detach().to(device=p.device, copy=True)
+                    want = v.dtype if v.dtype == torch.float8_e4m3fn else torch.float32
+                    self.state[p][k] = v.detach().to(device=p.device, dtype=want, copy=True)
         self._plan = None
 
     def flat_state(self) -> bool:

@@ -771,18 +771,22 @@ int launch_begin(const prl_list_entry* e, int64_t count, const prl_list_group* g
   }
 }
 
+// a launch has fewer than 2^32 threads: a batch ends before its workgroups pass this
+constexpr int64_t L_MAX_BLOCKS = (int64_t)1 << 23;
+
 int launch_adam32(const prl_list_entry* e, int64_t count, const Coef* coef, hipStream_t st) {
   Adam32Args a{};
   a.coef = coef;
   int64_t blocks = 0;
   for (int64_t i = 0; i <= count; ++i) {
-    if (a.count == L_BATCH || (i == count && a.count > 0)) {
+    const int64_t more = i < count && e[i].bits == 32 ? cdiv(e[i].numel, L_CHUNK32) : 0;
+    if (a.count > 0 && (a.count == L_BATCH || i == count || blocks + more > L_MAX_BLOCKS)) {
       hipLaunchKernelGGL(list_adam32_kernel, dim3((unsigned)blocks), dim3(L_THREADS), 0, st, a);
       PRL_LAUNCH_CHECK("list_adam32");
       blocks = 0;
       a.count = 0;
     }
-    if (i == count || e[i].numel == 0 || e[i].bits != 32) continue;
+    if (more == 0) continue;
     const int k = a.count++;
     a.param[k] = e[i].param;
     a.grad[k] = e[i].grad;
@@ -792,7 +796,7 @@ int launch_adam32(const prl_list_entry* e, int64_t count, const Coef* coef, hipS
     a.n[k] = e[i].numel;
     a.start[k] = (unsigned)blocks;
     a.which[k] = (unsigned)i | (unsigned)e[i].dtype << 30;
-    blocks += cdiv(e[i].numel, L_CHUNK32);
+    blocks += more;
   }
   return PRL_OK;
 }
@@ -802,13 +806,14 @@ int launch_adam8(const prl_list_entry* e, int64_t count, const Coef* coef, hipSt
   a.coef = coef;
   int64_t blocks = 0;
   for (int64_t i = 0; i <= count; ++i) {
-    if (a.count == L_BATCH8 || (i == count && a.count > 0)) {
+    const int64_t more = i < count && e[i].bits == 8 ? cdiv(e[i].numel, adam8_chunk_of((unsigned)e[i].dtype, e[i].master != nullptr)) : 0;
+    if (a.count > 0 && (a.count == L_BATCH8 || i == count || blocks + more > L_MAX_BLOCKS)) {
       hipLaunchKernelGGL(list_adam8_kernel, dim3((unsigned)blocks), dim3(L_THREADS), 0, st, a);
       PRL_LAUNCH_CHECK("list_adam8");
       blocks = 0;
       a.count = 0;
     }
-    if (i == count || e[i].numel == 0 || e[i].bits != 8) continue;
+    if (more == 0) continue;
     const int k = a.count++;
     a.param[k] = e[i].param;
     a.grad[k] = e[i].grad;
@@ -820,7 +825,7 @@ int launch_adam8(const prl_list_entry* e, int64_t count, const Coef* coef, hipSt
     a.n[k] = e[i].numel;
     a.start[k] = (unsigned)blocks;
     a.which[k] = (unsigned)i | (unsigned)e[i].dtype << 30;
-    blocks += cdiv(e[i].numel, adam8_chunk_of((unsigned)e[i].dtype, e[i].master != nullptr));
+    blocks += more;
   }
   return PRL_OK;
 }
@@ -922,6 +927,7 @@ extern "C" int prl_list_adamw(const prl_list_entry* entries, int64_t count, cons
   PRL_REQUIRE(n_groups >= 0 && (n_groups == 0 || groups), "prl_list_adamw: null groups");
   for (int64_t i = 0; i < count; ++i) {
     const prl_list_entry& e = entries[i];
+    PRL_REQUIRE(e.numel <= L_MAX_BLOCKS * L_CHUNK8, "prl_list_adamw: tensor %lld: bad size %lld", (long long)i, (long long)e.numel);
     PRL_REQUIRE(e.bits == 32 || e.bits == 8, "prl_list_adamw: tensor %lld: moments in %d bits", (long long)i, (int)e.bits);
     PRL_REQUIRE(e.group >= 0 && e.group < n_groups, "prl_list_adamw: tensor %lld: group %lld of %lld", (long long)i,
                 (long long)e.group, (long long)n_groups);

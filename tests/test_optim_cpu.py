@@ -39,7 +39,7 @@ def test_c_entry_refuses_bad_lists():
     ok = dict(param=4096, grad=8192, exp_avg=12288, second=16384, step=20480, numel=10)
     cases = [
         (dict(ok, dtype=3), "unknown type"), (dict(ok, dtype=-1), "unknown type"),
-        (dict(ok, numel=-1), "bad size"), (dict(ok, numel=1 << 40), "bad size"),
+        (dict(ok, numel=-1), "bad size"), (dict(ok, numel=1 << 40), "bad size"), (dict(ok, numel=(1 << 34) + 1), "bad size"),
         (dict(ok, bits=16), "moments in 16 bits"), (dict(ok, group=1), "group 1 of 1"), (dict(ok, group=-1), "group -1"),
         (dict(ok, step=0), "null step"), (dict(ok, grad=0), "null grad"), (dict(ok, param=0), "null pointer"),
         (dict(ok, second=0), "null pointer"), (dict(ok, bits=8), "null pointer"),

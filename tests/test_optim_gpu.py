@@ -211,7 +211,6 @@ def test_state_dict_round_trip(bits, dtype, master):
     params, grads = _make(SIZES, dtype, 6)
     a = _optim().AdamW(params, state_bits=bits, master=master)
     a.step()
-    saved = a.state_dict()
     kept = [p.detach().clone() for p in params]
     types = {k: v.dtype for k, v in a.state[params[4]].items()}
     a.step()
@@ -220,10 +219,8 @@ def test_state_dict_round_trip(bits, dtype, master):
         for p, k in zip(params, kept):
             p.copy_(k)
     b = _optim().AdamW(params, state_bits=bits, master=master)
-    # `saved` holds a's own tensors, which its second step moved: rebuild the first step's state
-    c = _optim().AdamW([torch.nn.Parameter(p.detach().clone()) for p in params], state_bits=bits, master=master)
-    del saved, c
-    fresh, fgrads = _make(SIZES, dtype, 6)
+    # (a.state_dict() holds a's own tensors, which its second step moved: the first step's state again)
+    fresh, _ = _make(SIZES, dtype, 6)
     d = _optim().AdamW(fresh, state_bits=bits, master=master)
     d.step()
     import copy
@@ -231,6 +228,30 @@ def test_state_dict_round_trip(bits, dtype, master):
     assert {k: v.dtype for k, v in b.state[params[4]].items()} == types
     b.step()
     assert all(torch.equal(p.detach(), w) for p, w in zip(params, want))
+
+
+def test_load_state_dict_of_other_adamws():
+    """A torch AdamW's 16-bit moments and host step counts become float32 on the device; amsgrad's and
+    maximize's are refused; moments of the other form by the next step."""
+    p = torch.nn.Parameter(torch.ones(40, device="cuda", dtype=torch.bfloat16))
+    q = torch.nn.Parameter(p.detach().clone())
+    p.grad, q.grad = torch.full_like(p, 0.5), torch.full_like(p, 0.5)
+    torch_opt = torch.optim.AdamW([q])
+    torch_opt.step()
+    opt = _optim().AdamW([p])
+    opt.load_state_dict(torch_opt.state_dict())
+    st = opt.state[p]
+    assert st["exp_avg"].dtype == torch.float32 and st["step"].is_cuda and float(st["step"]) == 1.0
+    assert torch.equal(st["exp_avg"], torch_opt.state[q]["exp_avg"].float())
+    opt.step()
+    assert float(st["step"]) == 2.0
+    for kw in (dict(amsgrad=True), dict(maximize=True)):
+        with pytest.raises(ValueError, match="amsgrad or maximize"):
+            _optim().AdamW([p]).load_state_dict(torch.optim.AdamW([q], **kw).state_dict())
+    other = _optim().AdamW([p], state_bits=8)
+    other.load_state_dict(opt.state_dict())
+    with pytest.raises(ValueError, match="exp_"):
+        other.step()
 
 
 # ---------------------------------------------------------------------------------- values that are not finite
@@ -359,8 +380,9 @@ def test_adamw_captured_step_replays_as_eager(bits):
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
+            alone = _optim().grad_norm(grads + grads * 20)     # a list of its own, in the long form
             a.step(max_norm=0.5)
-        sets.append((params, grads, twins, lr, a, b, graph, a.total_norm, torch.cuda.Stream()))
+        sets.append((params, grads, twins, lr, a, b, graph, (a.total_norm, alone), torch.cuda.Stream()))
     for r in range(4):
         for params, grads, twins, lr, a, b, graph, norm, s in sets:
             lr.fill_(1e-2 / (r + 1))
@@ -374,7 +396,8 @@ def test_adamw_captured_step_replays_as_eager(bits):
         for params, grads, twins, lr, a, b, graph, norm, s in sets:
             b.step(max_norm=0.5)
             torch.cuda.synchronize()
-            assert torch.equal(norm, b.total_norm)
+            assert torch.equal(norm[0], b.total_norm)
+            assert torch.equal(norm[1], _optim().grad_norm(grads + grads * 20))
             for p, q in zip(params, twins):
                 assert torch.equal(p, q)
                 sa, sb = a.state[p], b.state[q]
