@@ -472,8 +472,9 @@ def _learn(make_optimizer, use_graphs, use_fused=False, cont=False, mb=256):
     S = torch.randn(n, D, generator=gen, device="cuda")
     act = (torch.randn(n, A, generator=gen, device="cuda") if cont
            else torch.randint(0, A, (n,), generator=gen, device="cuda").float())
-    ppo.memory.push_device(S, act, torch.randn(n, generator=gen, device="cuda"),
-                           (torch.rand(n, generator=gen, device="cuda") < 0.01).float())
+    ppo._test_data = (S, act, torch.randn(n, generator=gen, device="cuda"),
+                      (torch.rand(n, generator=gen, device="cuda") < 0.01).float())
+    ppo.memory.push_device(*ppo._test_data)
     ppo.learn()
     torch.cuda.synchronize()
     return ppo
@@ -492,6 +493,14 @@ def test_learn_steps_through_the_list_adamw():
         assert torch.equal(p, q)
         assert torch.equal(engine.optimizer.state[p]["exp_avg"], plain.optimizer.state[q]["exp_avg"])
     assert float(engine.optimizer.state[p]["step"]) == 24.0
+    # the per-step path goes on from the engine's state
+    engine.use_fused = False
+    engine.memory.push_device(*engine._test_data)
+    engine.learn()
+    assert engine.last_update_path == "graph"
+    for p, q in zip(engine.policy.parameters(), plain.policy.parameters()):
+        assert float(engine.optimizer.state[p]["step"]) == 48.0 and bool(torch.isfinite(p).all())
+        assert 0.0 < float((p - q).detach().abs().max()) <= 2 * 24 * 1e-3
     native = _learn(lambda p: AdamW(p, lr=1e-3, state_bits=8), True, use_fused=True)
     assert native.last_update_path == "graph" and native._last_graphed.wide is not None
     graph = _learn(lambda p: AdamW(p, lr=1e-3, state_bits=8), True)
@@ -526,6 +535,109 @@ def test_learn_wide_policy_and_rnd_with_8_bit_moments():
             assert all(float(o.state[p]["step"]) == steps for p in g["params"])
     new = list(ppo.policy.parameters()) + list(ppo.rnd.pred_net.parameters())
     assert all(bool(torch.isfinite(p).all()) and not torch.equal(p, o) for p, o in zip(new, old))
+
+
+@pytest.mark.parametrize("long", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype,master", [(torch.float32, False), (torch.bfloat16, True), (torch.float16, False)])
+def test_nothing_around_the_tensors_is_written(bits, dtype, master, long):
+    """Parameters, masters, moments, codes and scales as views with other values before and behind them
+    (7 of each kind), at every alignment: those stay, in the one-launch form and in the long one."""
+    sizes = [1, 2, 3, 4, 5, 63, 255, 256, 257, 258, 1021, 4099] * (3 if long else 1)
+    gap, kinds = 7, {}
+
+    def lay(name, lengths, of, fill):
+        flat = torch.full((gap + sum(n + gap for n in lengths),), fill, device="cuda").to(of)
+        at, views = gap, []
+        for n in lengths:
+            views.append(flat[at:at + n])
+            at += n + gap
+        kinds[name] = (flat, lengths, flat.clone())
+        return views
+
+    blocks = [-(-n // 256) for n in sizes]
+    params = [torch.nn.Parameter(v) for v in lay("param", sizes, dtype, 0.5)]
+    opt = _optim().AdamW(params, state_bits=bits, master=master)
+    codes = torch.float8_e4m3fn
+    state = {"exp_avg": lay("exp_avg", sizes, torch.float32 if bits == 32 else codes, 0.25),
+             "exp_avg_sq" if bits == 32 else "exp_rms": lay("second", sizes, torch.float32 if bits == 32 else codes, 2.0)}
+    if bits == 8:
+        state["exp_avg_scale"] = lay("first scale", blocks, torch.float32, 0.125)
+        state["exp_rms_scale"] = lay("second scale", blocks, torch.float32, 0.5)
+    if master and dtype != torch.float32:
+        state["master"] = lay("master", sizes, torch.float32, 0.5)
+    for i, (p, g) in enumerate(zip(params, lay("grad", sizes, dtype, 1.0))):
+        p.grad = g
+        opt.state[p].update({k: v[i] for k, v in state.items()}, step=torch.full((), 3.0, device="cuda"))
+    opt.step(max_norm=1.0)
+    torch.cuda.synchronize()
+    for name, (flat, lengths, old) in kinds.items():
+        at = gap
+        inside = torch.zeros(flat.numel(), dtype=torch.bool, device="cuda")
+        for n in lengths:
+            inside[at:at + n] = True
+            at += n + gap
+        new, was = flat.float(), old.float()
+        assert torch.equal(new[~inside], was[~inside]), name
+        if name == "grad":
+            assert torch.equal(new, was)
+        elif name in ("param", "master", "first scale", "second scale") and flat.dtype == torch.float32:
+            # (a 16-bit parameter's step, below lr = 1e-3, may round back to 0.5)
+            assert bool((new[inside] != was[inside]).all()), name
+
+
+def test_empty_lists_and_parameters():
+    O = _optim()
+    e = torch.nn.Parameter(torch.empty(0, device="cuda"))
+    e.grad = torch.empty(0, device="cuda")
+    p = torch.nn.Parameter(torch.ones((), device="cuda"))        # 0-dim
+    for bits in (32, 8):
+        opt = O.AdamW([e, p], state_bits=bits)
+        opt.step(max_norm=1.0)                                    # p has no gradient
+        assert float(opt.total_norm) == 0.0 and float(opt.state[e]["step"]) == 1.0 and not opt.state.get(p)
+        p.grad = torch.full((), 3.0, device="cuda")
+        opt.step(max_norm=1.0)
+        assert float(opt.total_norm) == 3.0 and float(opt.state[p]["step"]) == 1.0
+        p.grad = None
+    q = torch.nn.Parameter(torch.ones(5, device="cuda"))
+    opt = O.AdamW([q])
+    opt.step(max_norm=1.0)
+    assert float(opt.total_norm) == 0.0 and not opt.state.get(q) and torch.equal(q.detach(), torch.ones_like(q))
+    opt.step()
+    assert opt.total_norm is None
+
+
+def test_replays_and_eager_steps_of_one_optimizer_alternate():
+    """A graph's step and eager ones share state and counts; an eager step with other gradients, or with
+    a parameter left out, does not disturb the graph's."""
+    params, grads = _make([300, 70], torch.float32, 31)
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    a, b = _optim().AdamW(params, state_bits=8), _optim().AdamW(twins, state_bits=8)
+
+    def eager(opt, ps, first_only):
+        ps[0].grad = grads[0] * 2.0
+        ps[1].grad = None if first_only else grads[1] * 0.5
+        opt.step(max_norm=1.0)
+
+    for o, ps in ((a, params), (b, twins)):
+        for p, g in zip(ps, grads):
+            p.grad = g
+        o.step(max_norm=1.0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step(max_norm=1.0)
+    for k in range(3):
+        graph.replay()
+        eager(a, params, k == 1)
+        torch.cuda.synchronize()
+        for p, g in zip(twins, grads):
+            p.grad = g
+        b.step(max_norm=1.0)
+        eager(b, twins, k == 1)
+        for p, q in zip(params, twins):
+            assert torch.equal(p, q)
+    assert float(a.state[params[0]]["step"]) == 7.0 and float(a.state[params[1]]["step"]) == 6.0
 
 
 def test_step_runs_torch_hooks_and_shows_in_the_profiler():
