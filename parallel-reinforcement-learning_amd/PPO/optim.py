@@ -30,8 +30,6 @@ _MOMENTS = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_rms", "exp_avg_sc
 _ptr, _numel, _contiguous, _device = (torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous,
                                       torch.Tensor.get_device)
 _dtype, _layout = attrgetter("dtype"), attrgetter("layout")
-
-
 _GLOBAL_HOOKS = [getattr(import_module("torch.optim.optimizer"), f"_global_optimizer_{k}_hooks", (True,))
                  for k in ("pre", "post")]
 
@@ -237,7 +235,7 @@ class AdamW(torch.optim.Optimizer):
         lr, (beta1, beta2), on_device = group["lr"], group["betas"], 0
         if torch.is_tensor(lr):
             if lr.is_cuda:
-                if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != group["params"][0].device:
+                if lr.dtype != torch.float32 or lr.numel() != 1 or any(p.device != lr.device for p in group["params"][:1]):
                     raise ValueError("a device lr must be one float32 value on the parameters' device")
                 lr, on_device = 0.0, lr.data_ptr()
             else:
@@ -271,8 +269,9 @@ class _Plan:
             if not st:
                 opt._init_state(p, group, st)
             columns.append(opt._check_state(p, group, st))
-        if len(set(map(_ptr, (c[5] for c in columns)))) < len(columns):
-            raise ValueError("two parameters share a step count tensor: each needs its own")
+        own = [t.data_ptr() for c in columns for t in c if t is not None and t.numel()]
+        if len(set(own)) < len(own):
+            raise ValueError("two state tensors (or step counts) are the same memory: each parameter needs its own")
         self.values = list(chain.from_iterable(map(dict.values, opt.state.values())))
         self.dtypes, self.numels = list(map(_dtype, self.params)), list(map(_numel, self.params))
         self.tensors = self.params + [t for c in columns for t in c if t is not None]

@@ -1,7 +1,7 @@
 // prl_optim.hip — optimizer operators over lists of tensors (include/prl_optim.h): the global
 // gradient norm and one clipped AdamW step with 32-bit or 8-bit moments.
 //
-// The tensors' descriptors travel in the kernels' arguments, a batch of up to 64 tensors per launch:
+// The tensors' descriptors travel in the kernels' arguments, a batch of 48 to 256 tensors per launch:
 // a captured graph then holds them itself, and no table on the device has to outlive a call.  Every
 // tensor is cut into chunks of one workgroup each; a workgroup finds its tensor by comparing its
 // index with the batch's chunk prefix, 64 entries per ballot.  Fields that a uniform index reads
@@ -448,7 +448,8 @@ __device__ inline unsigned max_bits(const float (&x)[4]) {
 // within 2^-44 of the root before its last rounding.  Below 2^-126 it comes out small (a positive v
 // still gives a positive root), and an infinite v gives NaN: a block is taken again with sqrtf() unless its
 // largest root lies from 2^-40 to the largest finite number.  In such a block a root below 2^-63 is the
-// smallest code, right or small, and adds nothing to an eps of 2^-40 or more in the denominator.
+// smallest code, right or small, and vanishes beside an eps of 2^-30 or more in the denominator (beta2 up
+// to 1 - 2^-16); a smaller eps takes sqrtf() throughout.
 constexpr unsigned QUICK_FROM = 0x2b800000u;   // 2^-40
 __device__ inline float quick_root(float v) {
   const float y = __builtin_amdgcn_rsqf(fmaxf(v, 0x1p-126f));
@@ -509,8 +510,8 @@ __device__ inline void adam8_block(const Coef& c, PRL_GLOBAL typename T::One* p,
   }
   unsigned m_max = max_bits<true>(m), r_max = max_bits<false>(r);
   wave_max_pair(m_max, r_max);
-  // not the quick root's range (see there), or an eps that its error far below r_max could reach
-  if (r_max - QUICK_FROM >= 0x7f800000u - QUICK_FROM || c.eps < 0x1p-40f) {
+  // not the quick root's range (see there)
+  if (r_max - QUICK_FROM >= 0x7f800000u - QUICK_FROM || c.eps < 0x1p-30f) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) r[e] = sqrtf(v[e]);
     unsigned again = m_max;
@@ -955,6 +956,12 @@ extern "C" int prl_list_adamw(const prl_list_entry* entries, int64_t count, cons
   if (count == 0 && norm == nullptr) return PRL_OK;
   PRL_REQUIRE(norm == nullptr || max_norm >= 0.0f, "prl_list_adamw: max_norm %g", (double)max_norm);
   PRL_REQUIRE(n_groups >= 0 && (n_groups == 0 || groups), "prl_list_adamw: null groups");
+  for (int64_t g = 0; g < n_groups; ++g) {
+    const prl_list_group& h = groups[g];
+    PRL_REQUIRE(h.beta1 >= 0.0 && h.beta1 < 1.0 && h.beta2 >= 0.0 && h.beta2 < 1.0 && h.eps >= 0.0 &&
+                    h.weight_decay >= 0.0 && (h.lr_dev != nullptr || h.lr >= 0.0),
+                "prl_list_adamw: group %lld: lr, eps and weight_decay must not be negative, betas lie in [0, 1)", (long long)g);
+  }
   for (int64_t i = 0; i < count; ++i) {
     const prl_list_entry& e = entries[i];
     PRL_REQUIRE(e.numel <= L_MAX_BLOCKS * L_CHUNK8, "prl_list_adamw: tensor %lld: bad size %lld", (long long)i, (long long)e.numel);

@@ -55,6 +55,10 @@ def test_c_entry_refuses_bad_lists():
     assert _adamw(long, ws=(1 << 20) + 8)[0] == -1
     assert _adamw([list_entry(**ok)], norm=4096, max_norm=-1.0)[0] == -1
     assert _adamw([list_entry(**ok)], norm=4096, max_norm=float("nan"))[0] == -1
+    for bad in ((1e-3, 1.0, 0.9, 0.0, 0.0, 0), (1e-3, 0.9, -0.1, 0.0, 0.0, 0), (-1.0, 0.9, 0.9, 0.0, 0.0, 0), (1e-3, 0.9, 0.9, -1.0, 0.0, 0),
+                (1e-3, 0.9, 0.9, 0.0, -1.0, 0), (float("nan"), 0.9, 0.9, 0.0, 0.0, 0), (1e-3, 0.9, float("nan"), 0.0, 0.0, 0)):
+        assert _adamw([list_entry(**ok)], groups=(bad,))[0] == -1
+    assert _adamw([list_entry(**ok)], n_groups=-1)[0] == -1
     assert _adamw([])[0] == 0          # nothing to do, nothing launched
     import prl_native
     L = prl_native.lib()

@@ -360,6 +360,24 @@ def test_adamw8_second_moment_follows_smaller_gradients():
     assert abs(float(r[::2].mean()) / high - 1) < 0.25 and abs(float(r[1::2].mean()) / low - 1) < 0.25
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("betas,eps", [((0.9, 0.999), 1e-15), ((0.0, 0.0), 1e-8), ((0.5, 0.9), 0.0), ((0.99, 0.99999), 1e-3)])
+def test_adamw_other_hyper_parameters(bits, betas, eps):
+    """Betas of 0, an eps of 0 and ones below and above the quick root's bound, no decay: three steps with
+    gradients over six decades within a block (none of them 0: eps = 0)."""
+    hyper = (1e-3, betas, eps, 0.0)
+    gen = torch.Generator().manual_seed(9)
+    params = [torch.nn.Parameter((torch.randn(n, generator=gen) * 0.1).cuda()) for n in (700, 45000)]
+    opt = _optim().AdamW(params, lr=1e-3, betas=betas, eps=eps, weight_decay=0.0, state_bits=bits)
+    for t in (1, 2, 3):
+        for p in params:
+            g = torch.randn(p.numel(), generator=gen).clamp(min=0.1) * 10.0 ** (-6 * torch.rand(p.numel(), generator=gen))
+            p.grad = g.cuda()
+        before = _before(opt, params, bits, t == 1)
+        opt.step()
+        _check_step(opt, params, before, 1.0, t, hyper, bits)
+
+
 # ---------------------------------------------------------------------------------- streams, graphs, layouts
 @pytest.mark.parametrize("bits", [32, 8])
 def test_adamw_captured_step_replays_as_eager(bits):
@@ -739,8 +757,20 @@ def test_refusals_on_the_device():
     q.grad = torch.ones_like(q)
     two.step()
     two.state[q]["step"] = two.state[p]["step"]
-    with pytest.raises(ValueError, match="step count"):
+    with pytest.raises(ValueError, match="same memory"):
         two.step()
+    two.state[q]["step"] = two.state[p]["step"].clone()
+    two.step()
+    two.state[q]["exp_avg_sq"] = two.state[p]["exp_avg_sq"]
+    with pytest.raises(ValueError, match="same memory"):
+        two.step()
+    odd = O.AdamW([q])
+    odd.param_groups[0]["betas"] = (0.9, 1.0)
+    with pytest.raises(RuntimeError, match="betas"):
+        odd.step()
+    odd.param_groups[0].update(betas=(0.9, 0.99), lr=torch.ones((), dtype=torch.float64, device="cuda"))
+    with pytest.raises(ValueError, match="device lr"):
+        odd.step()
     fresh = O.AdamW([q])
     graph = torch.cuda.CUDAGraph()
     with pytest.raises(RuntimeError, match="outside it first"):
