@@ -16,9 +16,9 @@
 // Everything here is bound by memory but the shortest lists (launches) and 8-bit moments of 16-bit
 // weights (instructions).  MI355X, 3 states in turn, so that nothing comes from the caches:
 //   norm of 126 M bfloat16 values               40 us  6.2 TB/s
-//   step of 126 M float32 values (28 B each)   560 us  6.3 TB/s  (list_adam32; 652 us with norm and begin)
+//   step of 126 M float32 values (28 B each)   560 us  6.3 TB/s  (list_adam32; 650 us with norm and begin)
 //   8-bit moments, 126 M float32 (16 B)        339 us  6.0 TB/s  (list_adam8)
-//   8-bit moments, 126 M bfloat16 (10 B)       238 us  5.3 TB/s
+//   8-bit moments, 126 M bfloat16 (10 B)       226 us  5.6 TB/s
 // (a 2 GiB tensor multiplied in place by torch: 5.9 TB/s).
 #include "prl_common.h"
 #include "../../include/prl_optim.h"
@@ -40,10 +40,10 @@ constexpr int L_BATCH = 64;           // of the 32-bit step,
 constexpr int L_BATCH8 = 48;          // of the 8-bit step (more pointers each),
 constexpr int L_BATCH_BEGIN = 256;    // of list_begin_kernel: as many as 4 KB of arguments hold
 constexpr int L_GROUPS = 16;
-// Values per workgroup of a step.  32 bits: 2,048 (50 M bfloat16 values with masters 255 us; 4,096: 260,
+// Values per workgroup of a step.  32 bits: 2,048 (50 M bfloat16 values with masters, clipped, 255 us; 4,096: 260,
 // 8,192: 266).  8 bits: 2,048 of float32 weights or masters (126 M values 336 us; 1,024: 351, 4,096: 350),
 // 4,096 of 16-bit weights alone, where the instructions count and with them what a workgroup
-// does once (126 M values 286 us; 1,024: 352, 2,048: 302).
+// does once (126 M values, clipped, 256 us; 2,048: 286, 8,192: 258).
 constexpr int L_CHUNK32 = 2048, L_CHUNK8 = 2048, L_CHUNK8_16 = 4096;
 constexpr int L_COEF = 12;            // floats per tensor in the workspace
 constexpr int L_NORM_BLOCKS = 2048;   // partial sums of a norm, besides one per tensor
@@ -386,7 +386,7 @@ __global__ __launch_bounds__(L_THREADS) void list_adam32_kernel(const Adam32Args
 
 // ---- the step, 8-bit moments -------------------------------------------------------------------
 // A block of 256 values is one wave's: 4 consecutive values per lane, so a code quad is one 32-bit
-// word, the block's largest magnitude a wave reduction, and nothing crosses waves.  Some 65 issue slots
+// word, the block's largest magnitude a wave reduction, and nothing crosses waves.  Some 60 issue slots
 // per value: beside 16 bytes (float32 weights) the loads bound it, beside 10 (16-bit weights) the
 // instructions do.  Rounding r to 8 bits to the nearest would leave it in place for good: a step moves it
 // by 0.05 % at beta2 = 0.999, codes lie 6 to 12 % apart, so it is rounded stochastically.
@@ -457,10 +457,12 @@ __device__ inline float quick_root(float v) {
   return fmaf(fmaf(-s, s, v), 0.5f * y, s);
 }
 
-// 256 / A for a block's largest magnitude A given as its bits; 0: the block is held as zeros
+// 256 / A for a block's largest magnitude A given as its bits, by v_rcp_f32 and one step of Newton's
+// method (both operands' sizes stay normal); 0: the block is held as zeros
 __device__ inline float block_factor(unsigned max_bits) {
-  const float A = __uint_as_float(max_bits);
-  return max_bits < 0x7f800000u && A >= 0x1p-118f ? 256.0f / A : 0.0f;
+  const float A = __uint_as_float(max_bits), a = A * 0x1p-8f;
+  const float x = __builtin_amdgcn_rcpf(a);
+  return max_bits < 0x7f800000u && A >= 0x1p-118f ? fmaf(fmaf(-a, x, 1.0f), x, x) : 0.0f;
 }
 // A as stored: NaN where a value of the block is not finite
 __device__ inline float block_store(unsigned max_bits, float k) {
@@ -527,7 +529,7 @@ __device__ inline void adam8_block(const Coef& c, PRL_GLOBAL typename T::One* p,
     if (MASTER) store_part<F32>(w + i, left, x);
     store_part<T>(p + i, left, x);
   }
-  // both factors in one division: the first moment's in lane 0, the second's in lane 1
+  // both factors at once: the first moment's in lane 0, the second's in lane 1
   const float k = block_factor(lane & 1 ? r_max : m_max);
   const float km = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(k), 0));
   const float kr = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(k), 1));
@@ -546,13 +548,18 @@ __device__ inline void adam8_block(const Coef& c, PRL_GLOBAL typename T::One* p,
     mw = __builtin_amdgcn_cvt_sr_fp8_f32(y(2), draw(2), mw, 2);
     mw = __builtin_amdgcn_cvt_sr_fp8_f32(y(3), draw(3), mw, 3);
   }
-  if (kr > 0.0f) {   // an r above 0 stays above 0: 2^-9 is the smallest code
-    const auto y = [&](int e) { return r[e] > 0.0f ? fmaxf(r[e] * kr, 0x1p-9f) : 0.0f; };
+  if (kr > 0.0f) {
+    float y[4] = {r[0] * kr, r[1] * kr, r[2] * kr, r[3] * kr};
+    // an r above 0 stays above 0: 2^-9 is the smallest code.  Few blocks hold one that small.
+    if (__ballot(fminf(fminf(y[0], y[1]), fminf(y[2], y[3])) < 0x1p-9f) != 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = r[e] > 0.0f ? fmaxf(y[e], 0x1p-9f) : 0.0f;
+    }
     const auto draw = [&](int e) { return d[e] & 0xffff0000u; };
-    rw = __builtin_amdgcn_cvt_sr_fp8_f32(y(0), draw(0), rw, 0);
-    rw = __builtin_amdgcn_cvt_sr_fp8_f32(y(1), draw(1), rw, 1);
-    rw = __builtin_amdgcn_cvt_sr_fp8_f32(y(2), draw(2), rw, 2);
-    rw = __builtin_amdgcn_cvt_sr_fp8_f32(y(3), draw(3), rw, 3);
+    rw = __builtin_amdgcn_cvt_sr_fp8_f32(y[0], draw(0), rw, 0);
+    rw = __builtin_amdgcn_cvt_sr_fp8_f32(y[1], draw(1), rw, 1);
+    rw = __builtin_amdgcn_cvt_sr_fp8_f32(y[2], draw(2), rw, 2);
+    rw = __builtin_amdgcn_cvt_sr_fp8_f32(y[3], draw(3), rw, 3);
   }
   if (left >= 4) {
     PRL_STORE_NT(u32_u, mc + i, (unsigned)mw);
