@@ -378,8 +378,10 @@ class PPO:
 
     def _fused_engine(self):
         """The fused update engine for this policy / mini_batch (None: shape outside it, or an
-        optimizer whose state the engine does not hold: optim.AdamW with 8-bit moments)."""
-        if isinstance(self.optimizer, AdamW) and not self.optimizer.flat_state():
+        optimizer whose step is not the engine's: optim.AdamW with 8-bit moments, or not of
+        exactly the policy's parameters)."""
+        if isinstance(self.optimizer, AdamW) and not self.optimizer.flat_state(
+                self.policy.parameters()):
             return None
         eng = getattr(self, "_engine", None)
         if eng is not None and eng.mini_batch == self.mini_batch_size:

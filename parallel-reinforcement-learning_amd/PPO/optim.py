@@ -177,13 +177,15 @@ class AdamW(torch.optim.Optimizer):
                     self.state[p][k] = v.detach().to(device=p.device, dtype=want, copy=True)
         self._plan = None
 
-    def flat_state(self) -> bool:
-        """Whether this optimizer's step is one AdamW step of float32 parameters with float32 moments
-        and one set of hyper-parameters: what the update engine runs inside its kernels."""
-        group = self.param_groups[0]
+    def flat_state(self, params) -> bool:
+        """Whether this optimizer's step is one AdamW step of exactly these parameters in float32, with
+        float32 moments and one set of hyper-parameters: what the update engine runs inside its
+        kernels."""
+        group, params = self.param_groups[0], list(params)
         return (len(self.param_groups) == 1 and group["state_bits"] == 32
-                and not torch.is_tensor(group["lr"])
-                and all(p.dtype == torch.float32 for p in group["params"]))
+                and not torch.is_tensor(group["lr"]) and len(params) == len(group["params"])
+                and all(map(is_, params, group["params"]))
+                and all(p.dtype == torch.float32 for p in params))
 
     def __setstate__(self, state):
         super().__setstate__(state)

@@ -519,6 +519,13 @@ def test_learn_steps_through_the_list_adamw():
     for p, q in zip(engine.policy.parameters(), plain.policy.parameters()):
         assert float(engine.optimizer.state[p]["step"]) == 48.0 and bool(torch.isfinite(p).all())
         assert 0.0 < float((p - q).detach().abs().max()) <= 2 * 24 * 1e-3
+    # an optimizer of some of the parameters is not the engine's: the others stay
+    part = _learn(lambda p: AdamW(list(p)[:4], lr=1e-3), True, use_fused=True)
+    torch.manual_seed(0)
+    from PPO import PPO
+    start = [p.detach().clone() for p in PPO(False, 4, 2).policy.parameters()]
+    moved = [not torch.equal(p, s) for p, s in zip(part.policy.parameters(), start)]
+    assert part.last_update_path == "graph" and moved == [i < 4 for i in range(len(start))]
     native = _learn(lambda p: AdamW(p, lr=1e-3, state_bits=8), True, use_fused=True)
     assert native.last_update_path == "graph" and native._last_graphed.wide is not None
     graph = _learn(lambda p: AdamW(p, lr=1e-3, state_bits=8), True)
@@ -724,6 +731,50 @@ def test_short_and_long_lists_agree():
         for r in runs:
             assert all(torch.equal(x, y) for x, y in zip(r, runs[0]))
             assert all(torch.equal(x, y.detach()) for x, y in zip(r, few[:32]))
+
+
+def _dp_worker(rank, world, port, out_dir, use_fused):
+    import os
+    import sys
+    from test_distributed_cpu import PATHS, _shard
+    sys.path[:0] = PATHS
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    torch.distributed.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        from PPO import PPO
+        from PPO.optim import AdamW
+        torch.cuda.set_device(0)
+        torch.manual_seed(0)
+        p = PPO(False, 4, 2, lr=1e-3, k_epochs=4, batch_size=1, mini_batch_size=64)
+        p.show_progress, p.use_fused = False, use_fused
+        p.optimizer = AdamW(p.policy.parameters(), lr=1e-3, state_bits=8)
+        S, A, R, D = _shard(rank, 64, 5)
+        if rank == 1:      # one minibatch less: its last steps add zero gradients
+            S, A, R, D = (x[:-64] for x in (S, A, R, D))
+        p.memory.push_device(*(torch.from_numpy(x).cuda() for x in (S, A, R, D)))
+        p.learn()
+        torch.cuda.synchronize()
+        torch.save(dict(params=[q.detach().cpu() for q in p.policy.parameters()], path=p.last_update_path,
+                        replays=p.last_graph_replays, step=[float(p.optimizer.state[q]["step"]) for q in p.policy.parameters()],
+                        codes=[p.optimizer.state[q]["exp_rms"].float().cpu() for q in p.policy.parameters()]),
+                   os.path.join(out_dir, f"rank{rank}.pt"))
+    finally:
+        torch.distributed.destroy_process_group()
+
+
+@pytest.mark.parametrize("use_fused", [False, True])
+def test_data_parallel_learn_with_8_bit_moments(tmp_path, use_fused):
+    """Two ranks on one GPU (gloo) with shards of unequal length: the engine declines, the per-step paths
+    (autograd; the native gradient step) clip and step the all-reduced gradient, and both ranks end with
+    the same bits, codes included."""
+    import os
+    import torch.multiprocessing as mp
+    mp.spawn(_dp_worker, args=(2, 29671 + int(use_fused), str(tmp_path), use_fused), nprocs=2, join=True)
+    a, b = (torch.load(os.path.join(tmp_path, f"rank{r}.pt"), weights_only=True) for r in range(2))
+    assert a["path"] == b["path"] == "graph" and a["replays"] > 0
+    assert a["step"] == b["step"] == [20.0] * len(a["step"])
+    for x, y in zip(a["params"] + a["codes"], b["params"] + b["codes"]):
+        assert torch.equal(x, y) and bool(torch.isfinite(x).all())
 
 
 def test_refusals_on_the_device():
