@@ -187,6 +187,14 @@ class AdamW(torch.optim.Optimizer):
                 and all(map(is_, params, group["params"]))
                 and all(p.dtype == torch.float32 for p in params))
 
+    def steps_exactly(self, params) -> bool:
+        """Whether the parameters with gradients are the same here and in params: step(max_norm=..) then
+        clips by the norm of params' gradients."""
+        own, params = [p for group in self.param_groups for p in group["params"]], list(params)
+        if len(own) == len(params) and all(map(is_, own, params)):
+            return True
+        return {id(p) for p in own if p.grad is not None} == {id(p) for p in params if p.grad is not None}
+
     def __setstate__(self, state):
         super().__setstate__(state)
         self._plan, self.total_norm = None, None
@@ -324,9 +332,9 @@ class _Plan:
 
 
 def clip_and_step(optimizer, params, max_norm: float) -> None:
-    """nn.utils.clip_grad_norm_(params, max_norm) + optimizer.step() (PPO.py:248-250); in one call
-    for this module's AdamW."""
-    if isinstance(optimizer, AdamW):
+    """nn.utils.clip_grad_norm_(params, max_norm) + optimizer.step() (PPO.py:248-250); in one call (the
+    gradients stay unclipped) for this module's AdamW if it steps exactly the gradients of params."""
+    if isinstance(optimizer, AdamW) and optimizer.steps_exactly(params):
         optimizer.step(max_norm=max_norm)
     else:
         nn.utils.clip_grad_norm_(params, max_norm)

@@ -110,6 +110,26 @@ def test_learn_keeps_its_step_for_other_optimizers():
     assert torch.equal(p, q) and torch.equal(p.grad, q.grad)
 
 
+@pytest.mark.parametrize("held,fused", [((0, 1, 2), True), ((2, 0, 1), True), ((0, 1, 2, 4), True), ((0, 1, 2, 3), False), ((0, 1), False)])
+def test_clip_and_step_takes_one_call_only_for_exactly_these_gradients(monkeypatch, held, fused):
+    """The list AdamW clips by the norm of all it holds: parameters 0 - 2 are clipped in its step only if these
+    are all that have a gradient in it (4 has none); else their gradients are, by their own norm."""
+    from PPO.optim import AdamW, clip_and_step
+    params = [torch.nn.Parameter(torch.ones(4)) for _ in range(5)]
+    for i, p in enumerate(params[:4]):
+        p.grad = torch.full((4,), 3.0 + i)
+    opt = AdamW([params[i] for i in held])
+    calls = []
+    monkeypatch.setattr(opt, "step", lambda **kw: calls.append(kw))
+    clip_and_step(opt, params[:3], 2.0)
+    assert calls == [{"max_norm": 2.0} if fused else {}]
+    want = [torch.full((4,), 3.0 + i) for i in range(4)]
+    if not fused:
+        c = 2.0 / (sum(4 * (3.0 + i) ** 2 for i in range(3)) ** 0.5 + 1e-6)
+        want[:3] = [g * c for g in want[:3]]
+    assert all(torch.allclose(p.grad, w, rtol=1e-6, atol=0.0) for p, w in zip(params, want))
+
+
 # ---------------------------------------------------------------------------------- the restatement itself
 def test_restatement_is_torch_adamw():
     gen = torch.Generator().manual_seed(0)

@@ -1,0 +1,104 @@
+"""The list AdamW (PPO/optim.py) inside learn() and beside the update engine: what is clipped by which
+norm, each step's values against the float64 restatement (optim_ref.py, with its per-value bounds),
+and optimizer state that changes hands between the engine, the per-step paths and load_state_dict()."""
+import copy
+
+import pytest
+import torch
+
+import optim_ref as R
+from test_optim_gpu import _before, _check_step
+
+pytestmark = pytest.mark.gpu
+
+
+def _adamw():
+    from PPO.optim import AdamW
+    return AdamW
+
+
+def _ppo(make_optimizer, n=2037, k_epochs=3, mb=256, use_fused=False, use_graphs=False, **kw):
+    """A discrete 4-observation PPO (seeded), and n transitions to learn from."""
+    from PPO import PPO
+    torch.manual_seed(0)
+    ppo = PPO(False, 4, 2, lr=1e-3, k_epochs=k_epochs, batch_size=64, mini_batch_size=mb)
+    ppo.show_progress, ppo.use_fused, ppo.use_graphs = False, use_fused, use_graphs
+    for k, v in kw.items():
+        setattr(ppo, k, v)
+    if make_optimizer is not None:
+        ppo.optimizer = make_optimizer(list(ppo.policy.parameters()))
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    data = (torch.randn(n, 4, generator=gen, device="cuda"), torch.randint(0, 2, (n,), generator=gen, device="cuda").float(),
+            torch.randn(n, generator=gen, device="cuda"), (torch.rand(n, generator=gen, device="cuda") < 0.01).float())
+    return ppo, data
+
+
+def _learn(ppo, data):
+    ppo.memory.push_device(*data)
+    ppo.learn()
+    torch.cuda.synchronize()
+    return ppo
+
+
+# ---------------------------------------------------------------------------------- the clipping norm
+def test_clip_and_step_clips_by_the_norm_of_the_given_parameters():
+    """An optimizer of some of the parameters, and one of more than these: the norm is the parameters', theirs
+    are the gradients clipped, value by value.  torch's norm is a float32 sum of n squares: off by at
+    most (n + 2) / 2 roundings, its coefficient by 3 more."""
+    from PPO.optim import clip_and_step
+    gen = torch.Generator().manual_seed(0)
+    hyper = (1e-2, (0.9, 0.999), 1e-8, 0.1)
+    for of in ((0, 1), (0, 1, 2, 3), (2, 1, 0)):
+        params = [torch.nn.Parameter(torch.randn(n, generator=gen).cuda()) for n in (40, 300, 90, 70)]
+        raw = [(torch.randn(p.numel(), generator=gen) * s).cuda() for p, s in zip(params, (1.0, 3.0, 40.0, 9.0))]
+        for p, g in zip(params, raw):
+            p.grad = g.clone()
+        opt = _adamw()([params[i] for i in of], lr=hyper[0], betas=hyper[1], eps=hyper[2], weight_decay=hyper[3])
+        old = [p.detach().clone() for p in params]
+        clipped = params[:3]
+        norm = R.norm64(raw[:3])
+        c = R.clip64(norm, 2.0)
+        assert c < 0.01
+        n = sum(p.numel() for p in clipped)
+        clip_and_step(opt, clipped, 2.0)
+        for i, (p, g, w) in enumerate(zip(params, raw, old)):
+            if i not in of:
+                assert torch.equal(p.detach(), w) and not opt.state.get(p)
+                continue
+            ci = c if i < 3 else 1.0
+            w1, m1, v1, ew, em, ev = R.step64(w.cpu().double(), g.cpu().double(), torch.zeros(p.numel()).double(),
+                                              torch.zeros(p.numel()).double(), 1, *hyper, ci)
+            rel = ((n + 2) / 2 + 3) * R.U32
+            st = opt.state[p]
+            assert bool(((st["exp_avg"].cpu().double() - m1).abs() <= em + rel * m1.abs()).all()), (of, i)
+            assert bool(((st["exp_avg_sq"].cpu().double() - v1).abs() <= ev + 2 * rel * v1).all()), (of, i)
+            # m and sqrt(v) change by the same factor: the quotient by the eps beside it at most
+            part = hyper[0] * m1.abs() / (1 - 0.9) / ((v1 / (1 - 0.999)).sqrt() + hyper[2])
+            assert bool(((p.detach().cpu().double() - w1).abs() <= ew + rel * part).all()), (of, i)
+
+
+def test_learn_with_an_optimizer_of_some_parameters_is_torchs():
+    """One step of learn() with an AdamW of the first four tensors, the gradients large enough to be clipped:
+    the gradients left behind are those of the same run with torch's AdamW bit for bit, the parameters both
+    float32 evaluations of one step from them."""
+    runs = []
+    for cls in (_adamw(), torch.optim.AdamW):
+        ppo, data = _ppo(lambda ps: cls(ps[:4], lr=1e-3), n=200, k_epochs=1, value_coef=300.0)
+        start = [p.detach().clone() for p in ppo.policy.parameters()]
+        runs.append((_learn(ppo, data), start))
+    (a, start), (b, again) = runs
+    assert all(torch.equal(x, y) for x, y in zip(start, again))
+    ours, theirs = list(a.policy.parameters()), list(b.policy.parameters())
+    total = R.norm64([p.grad for p in theirs])
+    assert abs(total - 2.0) < 1e-3                   # clipped
+    assert R.norm64([p.grad for p in theirs[:4]]) < 0.999 * total     # by more than the four's norm
+    for i, (p, q, w) in enumerate(zip(ours, theirs, start)):
+        assert torch.equal(p.grad, q.grad), i
+        if i >= 4:
+            assert torch.equal(p, w) and torch.equal(q, w)
+            continue
+        zero = torch.zeros(p.numel(), dtype=torch.float64)
+        w1, _, _, ew, _, _ = R.step64(w.reshape(-1).cpu().double(), p.grad.reshape(-1).cpu().double(), zero, zero, 1, 1e-3,
+                                      (0.9, 0.999), 1e-8, 1e-2, 1.0)
+        for x in (p, q):
+            assert bool(((x.detach().reshape(-1).cpu().double() - w1).abs() <= ew).all()), i
