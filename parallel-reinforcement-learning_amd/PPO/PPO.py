@@ -405,6 +405,7 @@ class PPO:
         if self._fused_path(world) and S.is_cuda:
             eng = self._fused_engine()
             if eng is not None:
+                eng.prepare()
                 if world == 1:
                     self.last_loss = eng.run(S, A, old_logp, adv, returns, self.k_epochs).clone()
                     self.last_update_path = "fused"

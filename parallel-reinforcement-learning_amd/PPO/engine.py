@@ -57,6 +57,7 @@ class FusedUpdate:
         """Alias parameters and optimizer state onto the flat buffers (copies current values)."""
         opt = self.ppo.optimizer
         self._opt = opt   # the optimizer these moments belong to (a replaced one re-binds)
+        self._synced = False     # whether the optimizer's state has been made the engine's
         with torch.no_grad():
             self.step.zero_()
             for p, fv, mv, vv in zip(self.params, self._views(self.flat), self._views(self.m),
@@ -75,12 +76,33 @@ class FusedUpdate:
         self._opt_views = (self._views(self.m), self._views(self.v))
 
     def bound(self) -> bool:
-        """True while the policy parameters still live in the flat buffer and the optimizer is
-        the one the moments were taken from."""
-        if self.ppo.optimizer is not self._opt:
+        """True while the policy parameters still live in the flat buffer, the optimizer is the one
+        the moments were taken from, and its state is still these buffers' views (not loaded,
+        replaced or emptied since)."""
+        opt = self.ppo.optimizer
+        if opt is not self._opt:
             return False
-        return all(p.data.data_ptr() == fv.data_ptr()
-                   for p, fv in zip(self.params, self._views(self.flat)))
+        for p, fv, mv, vv in zip(self.params, self._views(self.flat), *self._opt_views):
+            if p.data.data_ptr() != fv.data_ptr():
+                return False
+            st = opt.state.get(p)
+            if st and "exp_avg" in st:
+                if (st["exp_avg"].data_ptr() != mv.data_ptr()
+                        or st["exp_avg_sq"].data_ptr() != vv.data_ptr()):
+                    return False
+            elif self._synced:
+                return False
+        return True
+
+    def prepare(self):
+        """Before a learn's update: re-bind if the parameters or the optimizer's state were replaced,
+        else take the optimizer's step count (steps may have been taken outside the engine)."""
+        if not self.bound():
+            self._bind()
+            return
+        st = self.ppo.optimizer.state.get(self.params[0])
+        if st and "step" in st:
+            self.step.copy_(torch.as_tensor(st["step"], dtype=torch.float32).reshape(1))
 
     def _sync_optimizer_state(self):
         """Make the optimizer's state the engine's: moments as views, step counts = engine's."""
@@ -95,6 +117,7 @@ class FusedUpdate:
             else:
                 st["step"] = (self.step.reshape(()).clone() if on_device
                               else torch.tensor(float(self.step.item())))
+        self._synced = True
 
     def evaluate(self, module, S, A):
         """module.get_evaluate(S, A)'s log_prob and value for all rows (module: policy_old, same

@@ -102,3 +102,56 @@ def test_learn_with_an_optimizer_of_some_parameters_is_torchs():
                                       (0.9, 0.999), 1e-8, 1e-2, 1.0)
         for x in (p, q):
             assert bool(((x.detach().reshape(-1).cpu().double() - w1).abs() <= ew).all()), i
+
+
+# ---------------------------------------------------------------------------------- the engine and the optimizer's state
+def _same(a, b, steps):
+    for p, q in zip(a.policy.parameters(), b.policy.parameters()):
+        assert torch.equal(p, q)
+        for k in ("exp_avg", "exp_avg_sq"):
+            assert torch.equal(a.optimizer.state[p][k], b.optimizer.state[q][k]), k
+        assert float(a.optimizer.state[p]["step"]) == float(b.optimizer.state[q]["step"]) == steps
+
+
+@pytest.mark.parametrize("torchs", [False, True])
+def test_engine_goes_on_from_steps_taken_outside_it(torchs):
+    """Engine -> per-step path -> engine, for this AdamW and torch's: the engine goes on as one that is
+    built from the optimizer's state there."""
+    make = None if torchs else lambda ps: _adamw()(ps, lr=1e-3)
+    runs = []
+    for fresh in (False, True):
+        ppo, data = _ppo(make, use_fused=True, use_graphs=True)
+        for k, path in enumerate(("fused", "graph", "fused")):
+            ppo.use_fused = path == "fused"
+            if fresh and k == 2:
+                ppo._engine = None
+            _learn(ppo, data)
+            assert ppo.last_update_path == path
+        runs.append(ppo)
+    _same(*runs, 72.0)
+
+
+@pytest.mark.parametrize("torchs", [False, True])
+def test_engine_takes_loaded_state(torchs):
+    """load_state_dict() on an optimizer whose state the engine holds: the next learn() starts from what was
+    loaded, as an engine built after the load does; an emptied state starts from nothing."""
+    make = None if torchs else lambda ps: _adamw()(ps, lr=1e-3)
+    runs = []
+    for fresh in (False, True):
+        ppo, data = _ppo(make, use_fused=True)
+        _learn(ppo, data)
+        saved = copy.deepcopy(ppo.optimizer.state_dict())
+        _learn(ppo, data)
+        ppo.optimizer.load_state_dict(saved)
+        if fresh:
+            ppo._engine = None
+        _learn(ppo, data)
+        assert ppo.last_update_path == "fused"
+        runs.append(ppo)
+    _same(*runs, 48.0)
+    for ppo, fresh in zip(runs, (False, True)):
+        ppo.optimizer.state.clear()
+        if fresh:
+            ppo._engine = None
+        _learn(ppo, data)
+    _same(*runs, 24.0)
