@@ -179,13 +179,21 @@ class AdamW(torch.optim.Optimizer):
 
     def flat_state(self, params) -> bool:
         """Whether this optimizer's step is one AdamW step of exactly these parameters in float32, with
-        float32 moments and one set of hyper-parameters: what the update engine runs inside its
-        kernels."""
+        float32 moments (those in the state too, if there are any) and one set of hyper-parameters:
+        what the update engine runs inside its kernels."""
         group, params = self.param_groups[0], list(params)
-        return (len(self.param_groups) == 1 and group["state_bits"] == 32
+        if not (len(self.param_groups) == 1 and group["state_bits"] == 32
                 and not torch.is_tensor(group["lr"]) and len(params) == len(group["params"])
                 and all(map(is_, params, group["params"]))
-                and all(p.dtype == torch.float32 for p in params))
+                and all(p.dtype == torch.float32 for p in params)):
+            return False
+        try:
+            for p in params:
+                if self.state.get(p):
+                    self._check_state(p, group, self.state[p])
+        except ValueError:       # the per-step path's first step refuses it by name
+            return False
+        return True
 
     def steps_exactly(self, params) -> bool:
         """Whether the parameters with gradients are the same here and in params: step(max_norm=..) then

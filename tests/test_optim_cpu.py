@@ -130,6 +130,24 @@ def test_clip_and_step_takes_one_call_only_for_exactly_these_gradients(monkeypat
     assert all(torch.allclose(p.grad, w, rtol=1e-6, atol=0.0) for p, w in zip(params, want))
 
 
+def test_flat_state_looks_at_the_state():
+    """The engine is offered float32 moments only: state of the other form, of another size or incomplete is not
+    its business, whatever state_bits says; a parameter may have none yet."""
+    from PPO.optim import AdamW
+    p, q = torch.nn.Parameter(torch.ones(6)), torch.nn.Parameter(torch.ones(3))
+    opt = AdamW([p, q])
+    good = dict(step=torch.zeros(()), exp_avg=torch.zeros(6), exp_avg_sq=torch.zeros(6))
+    assert opt.flat_state([p, q])
+    opt.state[p] = dict(good)
+    assert opt.flat_state([p, q]) and not opt.flat_state([q, p]) and not opt.flat_state([p])
+    codes = torch.zeros(6, dtype=torch.float8_e4m3fn)
+    for bad in (dict(step=torch.zeros(()), exp_avg=codes, exp_rms=codes), dict(good, exp_avg=codes),
+                dict(good, exp_avg_sq=torch.zeros(5)), dict(good, exp_avg_sq=torch.zeros(6, dtype=torch.float64)),
+                {k: v for k, v in good.items() if k != "step"}):
+        opt.state[p] = bad
+        assert not opt.flat_state([p, q])
+
+
 # ---------------------------------------------------------------------------------- the restatement itself
 def test_restatement_is_torch_adamw():
     gen = torch.Generator().manual_seed(0)

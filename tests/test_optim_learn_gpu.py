@@ -155,3 +155,25 @@ def test_engine_takes_loaded_state(torchs):
             ppo._engine = None
         _learn(ppo, data)
     _same(*runs, 24.0)
+
+
+@pytest.mark.parametrize("held,bits", [(8, 32), (32, 8)])
+def test_learn_refuses_state_of_the_other_form(held, bits):
+    """State of 8-bit moments loaded into an optimizer of 32-bit ones, or the other way round: learn() refuses
+    it by the state's name as step() does, and leaves parameters and state as they were."""
+    ppo, data = _ppo(lambda ps: _adamw()(ps, lr=1e-3, state_bits=held), use_fused=True)
+    _learn(ppo, data)
+    other = _adamw()(ppo.policy.parameters(), lr=1e-3, state_bits=bits)
+    other.load_state_dict(copy.deepcopy(ppo.optimizer.state_dict()))
+    ppo.optimizer = other
+    params = [p.detach().clone() for p in ppo.policy.parameters()]
+    state = {p: {k: (t, t.clone()) for k, t in other.state[p].items()} for p in ppo.policy.parameters()}
+    for ppo.use_graphs in (True, False):
+        ppo.memory.push_device(*data)
+        with pytest.raises(ValueError, match="exp_"):
+            ppo.learn()
+        torch.cuda.synchronize()
+        for p, old in zip(ppo.policy.parameters(), params):
+            assert torch.equal(p.detach(), old) and other.state[p].keys() == state[p].keys()
+            for k, (t, was) in state[p].items():
+                assert other.state[p][k] is t and torch.equal(t.float(), was.float()), k
