@@ -246,6 +246,9 @@ class AdamW(torch.optim.Optimizer):
         table, keep = plan.fill(grads)
         self.total_norm = prl_native.list_adamw(table, array("q", words), plan.device,
                                                 None if max_norm is None else float(max_norm), plan.workspace)
+        # the kernels write through addresses: autograd is told, so that backward() on a graph from before
+        # this step is refused (some 60 ns a parameter)
+        torch.autograd.graph.increment_version(plan.params)
         return loss
 
     @staticmethod

@@ -827,3 +827,20 @@ def test_refusals_on_the_device():
     with pytest.raises(RuntimeError, match="outside it first"):
         with torch.cuda.graph(graph):
             fresh.step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_step_raises_the_parameters_versions(bits):
+    """A graph kept from before a step is refused by backward() after it, as with torch's AdamW; parameters
+    without a gradient keep their version."""
+    for make in (lambda ps: _optim().AdamW(ps, state_bits=bits), torch.optim.AdamW):
+        p, q, r = (torch.nn.Parameter(torch.randn(5, device="cuda")) for _ in range(3))
+        opt = make([p, q, r])
+        loss = (p * q).square().sum()
+        loss.backward(retain_graph=True)
+        for _ in range(2):                   # (the second: the list as it was laid out)
+            before = p._version, q._version, r._version
+            opt.step()
+            assert p._version > before[0] and q._version > before[1] and r._version == before[2]
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                loss.backward(retain_graph=True)
