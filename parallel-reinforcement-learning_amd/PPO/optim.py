@@ -48,6 +48,18 @@ def _dense(tensors, device, name):
     return tensors if all(map(_contiguous, tensors)) else [t.detach().contiguous() for t in tensors]
 
 
+def _refuse_shared(written):
+    """Refuses (kind, tensor) pairs of which two share memory: a value written by two workgroups would
+    be either's."""
+    spans = sorted((str(t.device), t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), kind)
+                   for kind, t in written if t.numel())
+    for a, b in zip(spans, spans[1:]):
+        if a[0] == b[0] and b[1] < a[2]:
+            if a[3] == b[3] == "a parameter":
+                raise ValueError("two parameters share memory (or one is listed twice)")
+            raise ValueError(f"{a[3]} and {b[3]} are (in part) the same memory: each needs its own")
+
+
 def grad_norm(tensors) -> torch.Tensor:
     """The global 2-norm of a list of device tensors (float32, bfloat16, float16, mixed as they
     are), as a 0-dim float32 tensor: sqrt of the sum of all squares, summed in float64 in a fixed
@@ -115,12 +127,7 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"parameters must be float32, bfloat16 or float16 (got {p.dtype})")
             if p.is_sparse or not p.is_contiguous():
                 raise ValueError("parameters must be dense and contiguous")
-        # a value stepped by two entries of a list would race
-        spans = sorted((str(p.device), p.data_ptr(), p.data_ptr() + p.numel() * p.element_size())
-                       for g in self.param_groups for p in g["params"] if p.numel())
-        for a, b in zip(spans, spans[1:]):
-            if a[0] == b[0] and b[1] < a[2]:
-                raise ValueError("two parameters share memory (or one is listed twice)")
+        _refuse_shared(("a parameter", p) for g in self.param_groups for p in g["params"])
 
     # ------------------------------------------------------------------ state
     def _init_state(self, p, group, st):
@@ -290,9 +297,8 @@ class _Plan:
             if not st:
                 opt._init_state(p, group, st)
             columns.append(opt._check_state(p, group, st))
-        own = [t.data_ptr() for c in columns for t in c if t is not None and t.numel()]
-        if len(set(own)) < len(own):
-            raise ValueError("two state tensors (or step counts) are the same memory: each parameter needs its own")
+        _refuse_shared(("a parameter" if k == 0 else "a state tensor", t)
+                       for p, c in zip(self.params, columns) for k, t in enumerate([p, *c]) if t is not None)
         self.values = list(chain.from_iterable(map(dict.values, opt.state.values())))
         self.dtypes, self.numels = list(map(_dtype, self.params)), list(map(_numel, self.params))
         self.tensors = self.params + [t for c in columns for t in c if t is not None]

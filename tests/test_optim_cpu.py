@@ -148,6 +148,59 @@ def test_flat_state_looks_at_the_state():
         assert not opt.flat_state([p, q])
 
 
+def _laid_out(monkeypatch, opt):
+    """What a step checks before anything is launched, for parameters on the CPU."""
+    import PPO.optim as O
+    monkeypatch.setattr(O, "_dense", lambda tensors, device, name: tensors)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    params = [p for g in opt.param_groups for p in g["params"]]
+    return O._Plan(opt, opt.param_groups, params, [p.grad for p in params])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_list_whose_written_tensors_overlap_is_not_laid_out(monkeypatch, bits):
+    """Parameters moved onto each other after the optimizer was made, and state that overlaps state or a
+    parameter in any part, are refused; neighbours without a gap are not."""
+    from PPO.optim import AdamW
+
+    def make():
+        flat = torch.ones(600)
+        params = [torch.nn.Parameter(flat[:300]), torch.nn.Parameter(flat[300:])]
+        for p in params:
+            p.grad = torch.ones(300)
+        opt = AdamW(params, state_bits=bits)
+        _laid_out(monkeypatch, opt)                  # makes the state
+        return opt, params, flat
+
+    opt, params, flat = make()
+    _laid_out(monkeypatch, opt)
+    params[1].data = flat[299:599]
+    with pytest.raises(ValueError, match="share memory"):
+        _laid_out(monkeypatch, opt)
+    params[1].data = flat[300:]
+    _laid_out(monkeypatch, opt)
+    second = "exp_avg_sq" if bits == 32 else "exp_rms"
+    whole = torch.zeros(600).to(opt.state[params[0]]["exp_avg"].dtype)
+    for one, two in (((0, "exp_avg"), (1, "exp_avg")), ((0, "exp_avg"), (0, second)), ((1, second), (0, "exp_avg"))):
+        for at, shared in ((299, True), (300, False)):
+            opt, params, flat = make()
+            for (i, k), lo in ((one, 0), (two, at)):
+                opt.state[params[i]][k] = whole[lo:lo + 300]
+            if shared:
+                with pytest.raises(ValueError, match="same memory"):
+                    _laid_out(monkeypatch, opt)
+            else:
+                _laid_out(monkeypatch, opt)
+    opt, params, flat = make()
+    opt.state[params[0]]["step"] = flat[10:11].view(())
+    with pytest.raises(ValueError, match="a parameter and a state tensor are"):
+        _laid_out(monkeypatch, opt)
+    opt, params, flat = make()
+    opt.state[params[0]]["step"] = opt.state[params[1]]["step"]
+    with pytest.raises(ValueError, match="same memory"):
+        _laid_out(monkeypatch, opt)
+
+
 # ---------------------------------------------------------------------------------- the restatement itself
 def test_restatement_is_torch_adamw():
     gen = torch.Generator().manual_seed(0)

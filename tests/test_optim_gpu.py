@@ -844,3 +844,21 @@ def test_step_raises_the_parameters_versions(bits):
             assert p._version > before[0] and q._version > before[1] and r._version == before[2]
             with pytest.raises(RuntimeError, match="modified by an inplace operation"):
                 loss.backward(retain_graph=True)
+
+
+def test_parameters_moved_onto_each_other_are_refused():
+    """A step after p.data put a parameter over another's memory: refused before anything is launched."""
+    flat = torch.ones(600, device="cuda")
+    params = [torch.nn.Parameter(flat[:300]), torch.nn.Parameter(flat[300:])]
+    for p in params:
+        p.grad = torch.ones_like(p)
+    opt = _optim().AdamW(params)
+    opt.step()
+    params[1].data = flat[299:599]
+    old = flat.clone()
+    with pytest.raises(ValueError, match="share memory"):
+        opt.step()
+    assert torch.equal(flat, old) and float(opt.state[params[0]]["step"]) == 1.0
+    params[1].data = flat[300:]
+    opt.step()
+    assert float(opt.state[params[0]]["step"]) == 2.0 and not torch.equal(flat, old)
