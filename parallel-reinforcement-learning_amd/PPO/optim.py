@@ -241,16 +241,18 @@ class AdamW(torch.optim.Optimizer):
         groups = self.param_groups
         params = [p for group in groups for p in group["params"]]
         grads = [p.grad for p in params]
-        plan = self._plan
-        if plan is None or not plan.holds(groups, params, grads, self.state):
-            plan = self._plan = None     # (dropped first: laying out may refuse)
+        plan, filled = self._plan, None
+        if plan is not None and plan.holds(groups, params, grads, self.state):
+            filled = plan.fill(grads)
+        if filled is None:
+            self._plan = None     # (dropped first: laying out may refuse)
             plan = _Plan(self, groups, params, grads)
             if not plan.params:
                 self.total_norm = None if max_norm is None else torch.zeros((), device=params[0].device)
                 return loss
-            self._plan = plan
+            filled, self._plan = plan.fill(grads), plan
         words = b"".join(map(self._group_words, groups))
-        table, keep = plan.fill(grads)
+        table, keep = filled
         self.total_norm = prl_native.list_adamw(table, array("q", words), plan.device,
                                                 None if max_norm is None else float(max_norm), plan.workspace)
         # the kernels write through addresses: autograd is told, so that backward() on a graph from before
@@ -328,11 +330,12 @@ class _Plan:
                 and list(map(_ptr, self.tensors)) == self.at)     # (the types: by the gradients, in fill())
 
     def fill(self, grads):
-        """The table with the gradients' addresses, and the tensors that these are of."""
+        """The table with the gradients' addresses, and the tensors that these are of; None if their types
+        or sizes are not the parameters' (any more: the list is to be laid out, and checked, again)."""
         if len(grads) != len(self.params):
             grads = [g for g in grads if g is not None]
-        if list(map(_dtype, grads)) != self.dtypes:
-            raise ValueError("a gradient must be of its parameter's type")
+        if list(map(_dtype, grads)) != self.dtypes or list(map(_numel, grads)) != self.numels:
+            return None
         try:
             contiguous = all(map(_contiguous, grads))
         except RuntimeError:      # a sparse one: _dense says so
@@ -342,8 +345,6 @@ class _Plan:
         at = list(map(_ptr, grads))
         if at != self.grads_at:
             _dense(grads, self.device.index, "a gradient")
-            if list(map(_numel, grads)) != self.numels:
-                raise ValueError("a gradient must be of its parameter's size")
             self.grads_at, self.table[1::_WORDS] = at, array("q", at)
         return self.table, grads
 

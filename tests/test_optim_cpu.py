@@ -201,6 +201,28 @@ def test_a_list_whose_written_tensors_overlap_is_not_laid_out(monkeypatch, bits)
         _laid_out(monkeypatch, opt)
 
 
+def test_a_laid_out_list_does_not_serve_other_sizes_or_types(monkeypatch):
+    """Gradients that were cut short or changed their type where they lie: the list is to be laid out, and
+    checked, again."""
+    from PPO.optim import AdamW
+    p, q = torch.nn.Parameter(torch.ones(10)), torch.nn.Parameter(torch.ones(4))
+    p.grad, q.grad = torch.ones(10), torch.ones(4)
+    opt = AdamW([p, q])
+    plan = _laid_out(monkeypatch, opt)
+    grads = [p.grad, q.grad]
+    for _ in range(2):
+        table, keep = plan.fill(grads)
+        assert [table[1], table[12]] == [g.data_ptr() for g in grads]
+    at, whole = p.grad.data_ptr(), p.grad.data
+    p.grad.data = whole[:3]
+    assert p.grad.data_ptr() == at and plan.holds(opt.param_groups, [p, q], grads, opt.state)
+    assert plan.fill(grads) is None
+    with pytest.raises(ValueError, match="type and size"):
+        _laid_out(monkeypatch, opt)
+    assert plan.fill([whole.view(torch.bfloat16)[:10], q.grad]) is None
+    assert plan.fill([whole, q.grad]) is not None
+
+
 # ---------------------------------------------------------------------------------- the restatement itself
 def test_restatement_is_torch_adamw():
     gen = torch.Generator().manual_seed(0)

@@ -862,3 +862,27 @@ def test_parameters_moved_onto_each_other_are_refused():
     params[1].data = flat[300:]
     opt.step()
     assert float(opt.state[params[0]]["step"]) == 2.0 and not torch.equal(flat, old)
+
+
+def test_gradients_cut_short_and_types_changed_in_place():
+    """A gradient made shorter at its address is refused; a parameter that became another type at its address
+    (and got a gradient of that type) steps as that type."""
+    p = torch.nn.Parameter(torch.ones(40, device="cuda"))
+    p.grad = torch.full_like(p, 0.5)
+    opt = _optim().AdamW([p])
+    opt.step()
+    old, whole = p.detach().clone(), p.grad.data
+    p.grad.data = whole[:3]
+    with pytest.raises(ValueError, match="type and size"):
+        opt.step()
+    assert torch.equal(p.detach(), old) and float(opt.state[p]["step"]) == 1.0
+    p.grad.data = whole
+    opt.step()
+    at = p.data_ptr()
+    p.grad = None
+    p.data = p.data.view(torch.bfloat16)[:40].fill_(0.25)
+    p.grad = torch.full_like(p, 0.125)
+    assert p.data_ptr() == at and p.dtype == torch.bfloat16
+    before = _before(opt, [p], 32, False)
+    opt.step()
+    _check_step(opt, [p], before, 1.0, 3, (1e-3, (0.9, 0.999), 1e-8, 1e-2), 32)
