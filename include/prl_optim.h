@@ -65,7 +65,9 @@ int prl_list_norm(const prl_list_entry* entries, int64_t count, float* norm, voi
  * bits 8: with A = the largest |x| of a block of 256 (its scale), m and r = sqrt(v) are held as
  * e4m3 values q of x / A * 256, so x = q * A / 256.  Rounding is stochastic (to the upper neighbour
  * with probability equal to the way past the lower one, in 2^-16ths) with bits hashed from the
- * value's index and t, so a run repeats itself bit for bit.  An r above 0 is held as at least the
+ * value's index and t, so a run repeats itself bit for bit; for that, the step count of 8-bit
+ * moments does not stay at 2^24, where float32's whole numbers end, but goes on by the next
+ * float32 (t is then that, and its bits are hashed).  An r above 0 is held as at least the
  * smallest code.  A block with a value that is not finite gets the scale NaN: all its 256 moments
  * are NaN from then on.  One whose A is below 2^-118 is held as zeros. */
 int prl_list_adamw(const prl_list_entry* entries, int64_t count, const prl_list_group* groups,

@@ -86,7 +86,9 @@ class AdamW(torch.optim.Optimizer):
     blocks of 256 consecutive values share a float32 scale A, the largest magnitude in the block, and
     hold exp_avg, and exp_rms = sqrt(exp_avg_sq), as float8_e4m3fn of value / A * 256 with
     stochastic rounding (bits hashed from the index and the step count: the same run gives the same
-    bits).  A gradient that is not finite makes its whole block's moments NaN.
+    bits; past 2^24 steps, where a float32 count of 32-bit moments stays, theirs goes on by the next
+    float32).  A gradient that is not finite, or so large that its square is not, makes its whole
+    block's moments NaN.
 
     master=True: a float32 copy (`master` in the state) behind every 16-bit parameter takes the
     step, the parameter receives its rounding.  Without it a 16-bit parameter is read, stepped in

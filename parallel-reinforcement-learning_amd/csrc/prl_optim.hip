@@ -200,20 +200,25 @@ __device__ inline float clip_coef(float norm, float max_norm) {
   const float clip = max_norm / (norm + 1e-6f);
   return clip > 1.0f ? 1.0f : clip;   // a NaN stays
 }
-// b^t by squaring; its relative error grows to t * 2^-53, below float32's rounding for every count that a
-// float32 holds.  Latency before a step: the CartPole policy's one launch takes 7.8 us, 8.5 with pow().
+// b^t by squaring; its relative error grows to t * 2^-53, below float32's rounding up to t = 2^28 (b^t is
+// below 2^-23 there for any b up to 1 - 2^-24).  Latency before a step: the CartPole policy's one launch takes
+// 7.8 us, 8.5 with pow().
 __device__ inline double power(double b, float t) {
   double r = 1.0;
-  for (unsigned k = (unsigned)t; k != 0; k >>= 1) {
+  for (unsigned k = (unsigned)fminf(t, 0xffffff00p0f); k != 0; k >>= 1) {
     if (k & 1) r *= b;
     b *= b;
   }
   return r;
 }
-// advances the step count
-__device__ inline Coef next_coef(const prl_list_group& g, float* count, float clip) {
+// Advances the step count.  float32 counts whole steps up to 2^24 and stays there.  That is well for 32-bit
+// moments; with 8-bit ones (coded) the draws would be the same at every step from then on, and a second moment
+// beside a block's decaying largest one fall to half of what it should be.  Theirs goes on by the next float32, whose
+// bits are hashed in the count's place.
+__device__ inline Coef next_coef(const prl_list_group& g, float* count, bool coded, float clip) {
   const double lr = g.lr_dev != nullptr ? (double)g.lr_dev[0] : g.lr;
-  const float step = count[0] + 1.0f;
+  float step = count[0] + 1.0f;
+  if (coded && step == count[0] && step < 0x1.fffffep127f) step = __uint_as_float(__float_as_uint(step) + 1);
   count[0] = step;
   Coef c{};
   c.clip = clip;
@@ -224,14 +229,15 @@ __device__ inline Coef next_coef(const prl_list_group& g, float* count, float cl
   c.omb2 = (float)(1.0 - g.beta2);
   c.beta2 = (float)g.beta2;
   c.eps = (float)g.eps;
-  c.seed = (unsigned)(int64_t)step * 0x9E3779B1u;
+  c.seed = (step <= 0x1p24f ? (unsigned)step : __float_as_uint(step)) * 0x9E3779B1u;
   return c;
 }
 
 // ---- once per call: the norm's fold, the step counts, the per-tensor scalars -------------------
+constexpr unsigned CODED = 0x80;
 struct BeginArgs {
   float* step[L_BATCH_BEGIN];
-  unsigned char group[L_BATCH_BEGIN];
+  unsigned char group[L_BATCH_BEGIN];   // and CODED: moments in 8 bits
   prl_list_group groups[L_GROUPS];
   const double* partial;   // n_partial sums to fold into *norm, or n_partial < 0: *norm is ready
   float* norm;             // or NULL: no clipping
@@ -266,7 +272,8 @@ __global__ __launch_bounds__(1024) void list_begin_kernel(const BeginArgs a) {
   }
   if (t >= a.count) return;
   const float clip = a.norm != nullptr ? clip_coef(s_norm, a.max_norm) : 1.0f;
-  a.coef[t] = next_coef(a.groups[a.group[t]], a.step[t], clip);
+  const unsigned group = a.group[t];
+  a.coef[t] = next_coef(a.groups[group & ~CODED], a.step[t], (group & CODED) != 0, clip);
 }
 
 // ---- the step, 32-bit moments ------------------------------------------------------------------
@@ -689,7 +696,7 @@ __global__ __launch_bounds__(64 * L_SMALL_WAVES) void list_small_kernel(const Sm
   const auto entry = [&](int item) { return __popcll(__ballot(first <= (unsigned)item)) - 1; };
   // the scalars beside the norm's loads, by the wave with the fewest blocks
   if (STEP && wave == L_SMALL_WAVES - 1 && lane < a.count)
-    s_coef[lane] = next_coef(a.groups[a.kind[lane] >> 16], a.step[lane], 1.0f);
+    s_coef[lane] = next_coef(a.groups[a.kind[lane] >> 16], a.step[lane], (a.kind[lane] >> 8 & 0xff) == 8, 1.0f);
   if (a.norm != nullptr) {
     double acc = 0.0;
     for (int b = wave; b < a.items; b += 4 * L_SMALL_WAVES) {
@@ -804,7 +811,7 @@ int launch_begin(const prl_list_entry* e, int64_t count, const prl_list_group* g
       a.groups[n_of++] = groups[e[i].group];
     }
     a.step[a.count] = e[i].step;
-    a.group[a.count] = (unsigned char)g;
+    a.group[a.count] = (unsigned char)(g | (e[i].bits == 8 ? CODED : 0));
     ++a.count;
   }
 }

@@ -886,3 +886,69 @@ def test_gradients_cut_short_and_types_changed_in_place():
     before = _before(opt, [p], 32, False)
     opt.step()
     _check_step(opt, [p], before, 1.0, 3, (1e-3, (0.9, 0.999), 1e-8, 1e-2), 32)
+
+
+# ---------------------------------------------------------------------------------- step counts past 2^24
+def test_adamw8_draws_go_on_past_2_to_the_24_steps():
+    """float32 counts whole steps up to 2^24.  From there 8-bit moments go on by the next float32, whose bits
+    are hashed: the rounding is drawn anew at every step, and a second moment still follows the gradients
+    beside a block's decaying largest one (as in test_adamw8_second_moment_follows_smaller_gradients,
+    whose bounds these are).  32-bit moments need no
+    draws: their count stays, as torch's does."""
+    n, T = 1 << 16, 1500
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
+    opt = _optim().AdamW([p], lr=0.0, state_bits=8, weight_decay=0.0)
+    g = torch.ones(n, device="cuda")
+    p.grad = g
+    opt.step()
+    st = opt.state[p]
+    spike = torch.ones(n, device="cuda")
+    spike[::2] = 10.0
+    st["exp_rms_scale"].fill_(10.0)                     # as after many steps of `spike`
+    st["exp_rms"].copy_(spike * 25.6)
+    st["step"].fill_(2.0 ** 24 - 2)
+    counts = []
+    for k in range(T):
+        opt.step()
+        if k < 6:
+            counts.append(float(st["step"]))
+    assert counts == [2.0 ** 24 - 1, 2.0 ** 24, 2.0 ** 24 + 2, 2.0 ** 24 + 4, 2.0 ** 24 + 6, 2.0 ** 24 + 8]
+    r = st["exp_rms"].float() * st["exp_rms_scale"].repeat_interleave(256) / 256
+    keep = 0.999 ** T
+    high, low = math.sqrt(100 * keep + 1 - keep), 1.0
+    assert abs(float(r[::2].mean()) / high - 1) < 0.25 and abs(float(r[1::2].mean()) / low - 1) < 0.25
+    q = torch.nn.Parameter(torch.zeros(4, device="cuda"))
+    q.grad = torch.ones(4, device="cuda")
+    other = _optim().AdamW([q])
+    other.step()
+    other.state[q]["step"].fill_(2.0 ** 24)
+    other.step()
+    assert float(other.state[q]["step"]) == 2.0 ** 24
+
+
+@pytest.mark.parametrize("count,long", [(2.0 ** 24 - 1, False), (2.0 ** 24, False), (2.0 ** 25, True), (2.0 ** 40, True), (2.0 ** 70, False)])
+def test_adamw8_large_counts_step_as_defined(count, long):
+    """One step from a large count, in the one-launch form and the long one: the draws are those of the count's
+    bits past 2^24, the bias corrections 1."""
+    import struct
+    params, grads = _make([300, 1000] + ([40000] if long else []), torch.float32, 17)
+    opt = _optim().AdamW(params, lr=1e-3, state_bits=8)
+    opt.step()
+    for p in params:
+        opt.state[p]["step"].fill_(count)
+    before = _before(opt, params, 8, False)
+    opt.step()
+    for p, (w, g, m, v) in zip(params, before):
+        st = opt.state[p]
+        t = float(st["step"])
+        up = struct.unpack("I", struct.pack("f", count))[0] + 1
+        assert t == (count + 1 if count < 2.0 ** 24 else struct.unpack("f", struct.pack("I", up))[0])
+        w1, m1, v1, ew, em, ev = R.step64(w, g, m, v, t, 1e-3, (0.9, 0.999), 1e-8, 1e-2, 1.0)
+        assert bool(((p.detach().cpu().double() - w1).abs() <= ew).all())
+        dm, dr = R.draws(p.numel(), int(t) if t <= 2.0 ** 24 else up)
+        r1 = v1.sqrt()
+        er = ev / (2 * r1.clamp(min=1e-70)) + 2 * R.U32 * r1
+        for k, x, d, least, e in (("exp_avg", m1, dm, 0.0, em), ("exp_rms", r1, dr, 2.0 ** -9, er)):
+            _, q, low, high = R.quantise(x, d, least, e)
+            got = st[k].cpu().double()
+            assert bool(((got.abs() >= low) & (got.abs() <= high)).all()), (k, p.numel())
