@@ -953,6 +953,7 @@ extern "C" int prl_list_norm(const prl_list_entry* entries, int64_t count, float
                              int64_t workspace_bytes, void* stream) {
   if (int rc = check_list("prl_list_norm", entries, count)) return rc;
   PRL_REQUIRE(norm, "prl_list_norm: null norm");
+  PRL_REQUIRE((reinterpret_cast<uintptr_t>(norm) & 3u) == 0, "prl_list_norm: norm not aligned to its type");
   if (is_small(entries, count, 0)) return launch_small<false>(entries, count, nullptr, 0, 0.0f, norm, as_stream(stream));
   PRL_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= prl_list_workspace_bytes(entries, count, 0),
               "prl_list_norm: workspace null, too small or not 16-B aligned");
@@ -969,12 +970,15 @@ extern "C" int prl_list_adamw(const prl_list_entry* entries, int64_t count, cons
   if (int rc = check_list("prl_list_adamw", entries, count)) return rc;
   if (count == 0 && norm == nullptr) return PRL_OK;
   PRL_REQUIRE(norm == nullptr || max_norm >= 0.0f, "prl_list_adamw: max_norm %g", (double)max_norm);
+  PRL_REQUIRE((reinterpret_cast<uintptr_t>(norm) & 3u) == 0, "prl_list_adamw: norm not aligned to its type");
   PRL_REQUIRE(n_groups >= 0 && (n_groups == 0 || groups), "prl_list_adamw: null groups");
   for (int64_t g = 0; g < n_groups; ++g) {
     const prl_list_group& h = groups[g];
     PRL_REQUIRE(h.beta1 >= 0.0 && h.beta1 < 1.0 && h.beta2 >= 0.0 && h.beta2 < 1.0 && h.eps >= 0.0 &&
                     h.weight_decay >= 0.0 && (h.lr_dev != nullptr || h.lr >= 0.0),
                 "prl_list_adamw: group %lld: lr, eps and weight_decay must not be negative, betas lie in [0, 1)", (long long)g);
+    PRL_REQUIRE((reinterpret_cast<uintptr_t>(h.lr_dev) & 3u) == 0, "prl_list_adamw: group %lld: lr_dev not aligned to its type",
+                (long long)g);
   }
   for (int64_t i = 0; i < count; ++i) {
     const prl_list_entry& e = entries[i];

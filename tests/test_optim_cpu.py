@@ -77,6 +77,20 @@ def test_c_entry_refuses_bad_lists():
     assert "too large" in L.prl_last_error().decode()
 
 
+def test_c_entry_refuses_unaligned_norm_and_lr():
+    from prl_native import list_entry
+    import prl_native
+    L = prl_native.lib()
+    ok = list_entry(param=4096, grad=8192, exp_avg=12288, second=16384, step=20480, numel=10)
+    rc, msg = _adamw([ok], norm=4098)
+    assert rc == -1 and "norm not aligned" in msg
+    rc, msg = _adamw([ok], groups=((0.0, 0.9, 0.999, 1e-8, 0.0, 4097),))
+    assert rc == -1 and "lr_dev not aligned" in msg
+    table = array("q", ok)
+    assert L.prl_list_norm(table.buffer_info()[0], 1, 4097, None, 0, None) == -1
+    assert "norm not aligned" in L.prl_last_error().decode()
+
+
 def test_python_refusals():
     from PPO.optim import AdamW, grad_norm
     p = torch.nn.Parameter(torch.ones(6))
