@@ -250,7 +250,8 @@ class AdamW(torch.optim.Optimizer):
             self._plan = None     # (dropped first: laying out may refuse)
             plan = _Plan(self, groups, params, grads)
             if not plan.params:
-                self.total_norm = None if max_norm is None else torch.zeros((), device=params[0].device)
+                self.total_norm = None if max_norm is None else torch.zeros(
+                    (), dtype=torch.float32, device=params[0].device if params else None)
                 return loss
             filled, self._plan = plan.fill(grads), plan
         words = b"".join(map(self._group_words, groups))

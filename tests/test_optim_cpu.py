@@ -112,6 +112,20 @@ def test_python_refusals():
     assert torch.equal(p.detach(), torch.ones(6)) and not opt.state[p].get("exp_avg", None)
 
 
+def test_steps_of_nothing():
+    """No gradients, or no parameters at all: no step, a norm of 0 in float32 whatever torch's default type is."""
+    from PPO.optim import AdamW
+    torch.set_default_dtype(torch.float64)
+    try:
+        for params in ([torch.nn.Parameter(torch.ones(3))], [dict(params=[])]):
+            opt = AdamW(params)
+            assert opt.step() is None and opt.total_norm is None
+            assert opt.step(max_norm=1.0) is None
+            assert opt.total_norm.dtype == torch.float32 and opt.total_norm.shape == () and float(opt.total_norm) == 0.0
+    finally:
+        torch.set_default_dtype(torch.float32)
+
+
 def test_learn_keeps_its_step_for_other_optimizers():
     """clip_and_step is clip_grad_norm_ + step() for any optimizer that is not this AdamW."""
     from PPO.optim import clip_and_step
