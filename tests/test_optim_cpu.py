@@ -117,7 +117,7 @@ def test_steps_of_nothing():
     from PPO.optim import AdamW
     torch.set_default_dtype(torch.float64)
     try:
-        for params in ([torch.nn.Parameter(torch.ones(3))], [dict(params=[])]):
+        for params in ([torch.nn.Parameter(torch.ones(3, dtype=torch.float32))], [dict(params=[])]):
             opt = AdamW(params)
             assert opt.step() is None and opt.total_norm is None
             assert opt.step(max_norm=1.0) is None
