@@ -952,3 +952,72 @@ def test_adamw8_large_counts_step_as_defined(count, long):
             _, q, low, high = R.quantise(x, d, least, e)
             got = st[k].cpu().double()
             assert bool(((got.abs() >= low) & (got.abs() <= high)).all()), (k, p.numel())
+
+
+# ---------------------------------------------------------------------------------- the one-launch form, value by value
+SHORT = [1, 3, 4, 5, 255, 256, 257, 1023, 4097, 0, 17411, 777]     # 112 blocks of 256 in 12 tensors
+
+
+def _one_launch(opt):
+    import prl_native
+    return prl_native.list_workspace_bytes(opt._plan.table, len(opt.param_groups)) == 0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype,master", [(torch.float32, False), (torch.bfloat16, False),
+                                          (torch.bfloat16, True), (torch.float16, False),
+                                          (torch.float16, True)])
+@pytest.mark.parametrize("max_norm", [None, 0.5])
+def test_adamw_steps_in_one_launch(bits, dtype, master, max_norm):
+    """Three steps (the first from empty state) of a list that one launch takes, clipped (0 < c < 1) and not."""
+    params, grads = _make(SHORT, dtype, 13)
+    hyper = (1e-2, (0.9, 0.999), 1e-8, 0.1)
+    opt = _optim().AdamW(params, lr=hyper[0], betas=hyper[1], eps=hyper[2], weight_decay=hyper[3],
+                         state_bits=bits, master=master)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for t in (1, 2, 3):
+        before = _before(opt, params, bits, t == 1)
+        norm = R.norm64(grads)
+        opt.step(max_norm=max_norm)
+        assert _one_launch(opt)
+        if max_norm is not None:
+            assert norm > max_norm and abs(float(opt.total_norm) - norm) <= 1.01 * R.U32 * norm
+        _check_step(opt, params, before, R.clip64(norm, max_norm), t, hyper, bits)
+        for g in grads:
+            g.copy_(torch.randn(g.shape, generator=gen, device="cuda") * 0.03)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_groups_and_types_in_one_launch(bits):
+    """16 groups with hyper-parameters of their own, types and masters mixed, one group's lr on the device."""
+    groups, every = [], []
+    for i in range(16):
+        dtype = (torch.float32, torch.bfloat16, torch.float16)[i % 3]
+        params, _ = _make([1 + (37 * i + 11 * j) % 700 for j in range(2)], dtype, i, packed=i % 2 == 0)
+        lr = 1e-3 * (i + 1)
+        betas = (0.8 + 0.01 * i, 0.99)
+        groups.append(dict(params=params, lr=torch.full((), lr, device="cuda") if i == 4 else lr,
+                           betas=betas, weight_decay=0.01 * i, master=i % 2 == 1))
+        every.append((params, (float(torch.tensor(lr)) if i == 4 else lr, betas, 1e-8, 0.01 * i)))
+    opt = _optim().AdamW(groups, state_bits=bits)
+    for t in (1, 2):
+        norm = R.norm64([p.grad for params, _ in every for p in params])
+        befores = [_before(opt, params, bits, t == 1) for params, _ in every]
+        opt.step(max_norm=1.0)
+        assert _one_launch(opt) and norm > 1.0
+        for (params, hyper), before in zip(every, befores):
+            _check_step(opt, params, before, R.clip64(norm, 1.0), t, hyper, bits)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_clipped_step_at_the_one_launch_bound_and_past_it(bits):
+    """160 blocks in one launch, 161 in several: both clipped steps against the restatement."""
+    for sizes, short in (([160 * 256], True), ([160 * 256, 1], False)):
+        params, grads = _make(sizes, torch.float32, 4, lead=3)
+        hyper = (1e-3, (0.9, 0.999), 1e-8, 1e-2)
+        opt = _optim().AdamW(params, lr=hyper[0], betas=hyper[1], eps=hyper[2], weight_decay=hyper[3], state_bits=bits)
+        for t in (1, 2):
+            before, norm = _before(opt, params, bits, t == 1), R.norm64(grads)
+            opt.step(max_norm=0.25 * norm)
+            assert _one_launch(opt) == short
+            _check_step(opt, params, before, R.clip64(norm, 0.25 * norm), t, hyper, bits)

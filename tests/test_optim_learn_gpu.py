@@ -177,3 +177,72 @@ def test_learn_refuses_state_of_the_other_form(held, bits):
             assert torch.equal(p.detach(), old) and other.state[p].keys() == state[p].keys()
             for k, (t, was) in state[p].items():
                 assert other.state[p][k] is t and torch.equal(t.float(), was.float()), k
+
+
+# ---------------------------------------------------------------------------------- every step's values
+def _pin(opt, bits, hyper):
+    """Checks every eager step of `opt` value by value against one float64 step from what it found; returns
+    the list of the steps' clip coefficients."""
+    params, seen, found = [p for g in opt.param_groups for p in g["params"]], [], []
+
+    def pre(o, args, kwargs):
+        max_norm = kwargs.get("max_norm")
+        c = R.clip64(R.norm64([p.grad for p in params]), max_norm)
+        found.append((c, _before(o, params, bits, not o.state.get(params[0]))))
+
+    def post(o, args, kwargs):
+        c, before = found.pop()
+        seen.append(c)
+        _check_step(o, params, before, c, len(seen), hyper, bits)
+    opt.register_step_pre_hook(pre)
+    opt.register_step_post_hook(post)
+    return seen
+
+
+HYPER = (1e-3, (0.9, 0.999), 1e-8, 1e-2)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_each_step_of_learn_is_the_definitions(bits):
+    """The eager per-step path, some steps clipped: 24 steps of 13 tensors in the one-launch form."""
+    ppo, data = _ppo(lambda ps: _adamw()(ps, lr=1e-3, state_bits=bits), value_coef=5.0)
+    seen = _pin(ppo.optimizer, bits, HYPER)
+    _learn(ppo, data)
+    assert ppo.last_update_path == "eager" and len(seen) == 24 and min(seen) < 1.0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_each_step_of_the_wide_policy_and_rnd_is_the_definitions(bits):
+    """348 observations, 17 actions through the native gradient step (clipped by 2), and the RND predictor's
+    update (not clipped)."""
+    from PPO import PPO
+    torch.manual_seed(0)
+    ppo = PPO(True, 348, 17, action_scaling=1.0, k_epochs=2, batch_size=64, mini_batch_size=512, use_RND=True)
+    ppo.show_progress = False
+    ppo.optimizer = _adamw()(ppo.policy.parameters(), lr=1e-3, state_bits=bits)
+    ppo.rnd.optimizer = _adamw()(ppo.rnd.pred_net.parameters(), lr=1e-3, state_bits=bits)
+    policy, rnd = _pin(ppo.optimizer, bits, HYPER), _pin(ppo.rnd.optimizer, bits, HYPER)
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    n = 1100
+    _learn(ppo, (torch.randn(n, 348, generator=gen, device="cuda"), torch.randn(n, 17, generator=gen, device="cuda") * 0.1,
+                 torch.randn(n, generator=gen, device="cuda"), (torch.rand(n, generator=gen, device="cuda") < 0.01).float()))
+    assert ppo.last_update_path == "graph" and ppo._last_graphed.wide is not None
+    assert len(policy) == 6 and rnd == [1.0] * 3
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_step_of_some_parameters_is_the_eager_one(bits):
+    """learn() with an optimizer of the first four tensors, clipped by all parameters' norm, twice over: the
+    replayed graph leaves the eager path's bits."""
+    runs = []
+    for graphs in (False, True):
+        ppo, data = _ppo(lambda ps: _adamw()(ps[:4], lr=1e-3, state_bits=bits), use_graphs=graphs, value_coef=300.0)
+        for _ in range(2):
+            _learn(ppo, data)
+        assert ppo.last_update_path == ("graph" if graphs else "eager") and (ppo.last_graph_replays > 0) == graphs
+        runs.append(ppo)
+    for i, (p, q) in enumerate(zip(*(r.policy.parameters() for r in runs))):
+        assert torch.equal(p, q), i
+        if i < 4:
+            a, b = (r.optimizer.state[x] for r, x in zip(runs, (p, q)))
+            assert float(a["step"]) == 48.0 and all(torch.equal(a[k].float(), b[k].float()) for k in a), i
