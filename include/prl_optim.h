@@ -23,7 +23,8 @@ enum prl_list_dtype { PRL_LIST_F32 = 0, PRL_LIST_BF16 = 1, PRL_LIST_F16 = 2 };
 #define PRL_LIST_BLOCK 256
 
 /* One tensor of a list (host struct, pointers on the device).  Tensors are contiguous and need
- * only their element type's alignment.  numel == 0 is allowed (the tensor is skipped, its step
+ * only their element type's alignment.  What a call writes shares no memory with anything else of
+ * the call (entries may have one grad in common).  numel == 0 is allowed (the tensor is skipped, its step
  * count still advances). */
 typedef struct prl_list_entry {
   void* param;        /* [numel] of dtype */
@@ -48,7 +49,8 @@ typedef struct prl_list_group {   /* host */
 } prl_list_group;
 
 /* Workspace of the two calls below for a list of these sizes (prl_list_norm: n_groups 0); 0 for a
- * short list, which needs none (NULL will do); -1 for a list that they refuse.  It holds nothing
+ * short list, which needs none (NULL will do); -1 if the number of tensors or one of the sizes is out
+ * of range (nothing else of the list is looked at).  It holds nothing
  * between calls and needs no initial value; two calls that may run at once need one each. */
 int64_t prl_list_workspace_bytes(const prl_list_entry* entries, int64_t count, int64_t n_groups);
 

@@ -79,7 +79,8 @@ class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's step (decoupled weight decay; no amsgrad, no maximize) on device
     parameters, and clipping by the global norm in the same call: step(max_norm=2.0) does what
     nn.utils.clip_grad_norm_(params, 2.0) and step() do, except that p.grad is left unclipped;
-    the norm is then in `total_norm` (a 0-dim float32 device tensor).
+    the norm is then in `total_norm` (a 0-dim float32 device tensor).  `params` are all parameters of
+    this optimizer that have a gradient: see clip_and_step for any others.
 
     state_bits=32: exp_avg and exp_avg_sq in float32 whatever the parameter's type (state_dict() is
     torch's AdamW's for float32 parameters).  state_bits=8: 2 bytes of state per value instead of 8:
@@ -91,8 +92,14 @@ class AdamW(torch.optim.Optimizer):
     block's moments NaN.
 
     master=True: a float32 copy (`master` in the state) behind every 16-bit parameter takes the
-    step, the parameter receives its rounding.  Without it a 16-bit parameter is read, stepped in
-    float32 and rounded back.
+    step, the parameter receives its rounding.  It is made from the parameter at its first step;
+    weights that are loaded into the parameter later have to be copied into it too, or the next step
+    brings the old ones back.  Without masters a 16-bit parameter is read, stepped in float32 and
+    rounded back.
+
+    Parameters, state tensors and masters share no memory with each other (a step refuses it) or
+    with gradients; parameters may share a gradient.  A step raises the parameters' autograd versions
+    as any in-place operation does (a graph's replay does not, as with torch's optimizers).
 
     lr may be a float32 device tensor: a captured step then reads it at every replay.  The step
     count of every parameter lives on the device, so a step can be captured into a HIP graph once

@@ -16,9 +16,9 @@
 // Everything here is bound by memory but the shortest lists (launches) and 8-bit moments of 16-bit
 // weights (instructions).  MI355X, 3 states in turn, so that nothing comes from the caches:
 //   norm of 126 M bfloat16 values               40 us  6.2 TB/s
-//   step of 126 M float32 values (28 B each)   560 us  6.3 TB/s  (list_adam32; 650 us with norm and begin)
+//   step of 126 M float32 values (28 B each)   560 us  6.3 TB/s  (list_adam32; 655 us with norm and begin)
 //   8-bit moments, 126 M float32 (16 B)        339 us  6.0 TB/s  (list_adam8)
-//   8-bit moments, 126 M bfloat16 (10 B)       226 us  5.6 TB/s
+//   8-bit moments, 126 M bfloat16 (10 B)   226 - 239 us  5.3 - 5.6 TB/s (two cards)
 // (a 2 GiB tensor multiplied in place by torch: 5.9 TB/s).
 #include "prl_common.h"
 #include "../../include/prl_optim.h"
@@ -428,7 +428,10 @@ __device__ inline void wave_max_pair(unsigned& x, unsigned& y) {
   y = (unsigned)__builtin_amdgcn_readlane((int)v, 63);
 }
 
-// a value's two 16-bit draws at this step are the halves of h ^ (h >> 16), h = draw_bits(its index
+// The mixing of the bits is published: C. Wellons' search for 32-bit integer hashes of low bias found this pair of
+// multipliers for the shifts 16, 15, 16.  0x9E3779B1 and 0x85EBCA77 (a step count's and an index's high word's
+// factor) are primes that xxHash's specification lists.
+// A value's two 16-bit draws at this step are the halves of h ^ (h >> 16), h = draw_bits(its index
 // folded to 32 bits, ..): the low one for the first moment, the high one for the second
 __device__ inline unsigned draw_bits(unsigned at, unsigned seed) {
   unsigned h = at ^ seed;
@@ -623,10 +626,18 @@ __global__ __launch_bounds__(L_THREADS) void list_adam8_kernel(const Adam8Args a
 
 // ---- a short list in one launch ------------------------------------------------------------------
 // Up to L_SMALL_ITEMS blocks of 256 values in L_SMALL tensors: one workgroup of 16 waves, a block per
-// wave at a time, takes the norm, the scalars and the step.  Such a list's time is the launches':
-// 9,027 float32 values in 13 tensors, clipped, take 13.6 us per call (7.8 on the GPU) here and 28 in three
-// launches, 37,347 in 18 tensors 18 (17.4) and 31.  Past the bound one workgroup's loads take longer than
-// two more launches.
+// wave at a time, takes the norm, the scalars and the step.  Both ways, us per clipped step of 16 tensors as a call /
+// on the GPU alone (50 steps in one graph), one launch and three:
+//   blocks   float32 weights, 32 bits    bfloat16 weights, 8 bits
+//      48    18.6 /  7.8  26.7 /  7.8    20.9 / 10.5  29.9 /  8.9
+//     112    18.8 / 13.1  27.0 /  8.3    20.9 / 19.7  29.8 /  9.6
+//     160    18.7 / 17.6  26.9 /  8.4    27.9 / 26.7  29.9 / 10.5
+//     176    19.3 / 18.7  26.9 /  8.3    29.6 / 28.7  29.7 / 10.4
+//     304    30.2 / 29.8  26.8 /  8.4    47.6 / 46.8  29.7 / 11.1
+// (the norm alone: 160 blocks 14.4 / 4.4 and 19.4 / 4.1, 1,008 blocks 18.5 / 17.7 and 19.6 / 3.9.)  One bound for
+// all, just below where the slowest form's calls are level.  It is a bound for calls, whose time is mostly the
+// host's: on the GPU alone (a captured step, a stream that is behind) three launches are level at some 45 blocks
+// and ahead beyond.
 constexpr int L_SMALL = 32;
 constexpr int L_SMALL_ITEMS = 160;
 constexpr int L_SMALL_WAVES = 16;
