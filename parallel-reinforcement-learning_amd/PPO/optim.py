@@ -103,7 +103,8 @@ class AdamW(torch.optim.Optimizer):
 
     lr may be a float32 device tensor: a captured step then reads it at every replay.  The step
     count of every parameter lives on the device, so a step can be captured into a HIP graph once
-    every parameter has taken one step outside it (which lays out the state)."""
+    every parameter has taken one step outside it (which lays out the state).  A graph goes on with the
+    tensors it was captured with: load_state_dict() installs new ones, so capture again after it."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *,
                  state_bits: int = 32, master: bool = False):
@@ -214,7 +215,7 @@ class AdamW(torch.optim.Optimizer):
     def steps_exactly(self, params) -> bool:
         """Whether the parameters with gradients are the same here and in params: step(max_norm=..) then
         clips by the norm of params' gradients."""
-        own, params = [p for group in self.param_groups for p in group["params"]], list(params)
+        own = [p for group in self.param_groups for p in group["params"]]
         if len(own) == len(params) and all(map(is_, own, params)):
             return True
         return {id(p) for p in own if p.grad is not None} == {id(p) for p in params if p.grad is not None}
@@ -362,6 +363,7 @@ class _Plan:
 def clip_and_step(optimizer, params, max_norm: float) -> None:
     """nn.utils.clip_grad_norm_(params, max_norm) + optimizer.step() (PPO.py:248-250); in one call (the
     gradients stay unclipped) for this module's AdamW if it steps exactly the gradients of params."""
+    params = [params] if isinstance(params, torch.Tensor) else list(params)
     if isinstance(optimizer, AdamW) and optimizer.steps_exactly(params):
         optimizer.step(max_norm=max_norm)
     else:

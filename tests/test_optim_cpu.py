@@ -251,6 +251,25 @@ def test_a_laid_out_list_does_not_serve_other_sizes_or_types(monkeypatch):
     assert plan.fill([whole, q.grad]) is not None
 
 
+def test_clip_and_step_takes_what_clip_grad_norm_takes(monkeypatch):
+    """An iterator of parameters, or one tensor."""
+    from PPO.optim import AdamW, clip_and_step
+    for of, given in ((1, lambda ps: iter(ps)), (2, lambda ps: iter(ps)), (2, lambda ps: ps[0]), (1, lambda ps: ps[0])):
+        params = [torch.nn.Parameter(torch.ones(4)) for _ in range(2)]
+        for p in params:
+            p.grad = torch.full((4,), 3.0)
+        opt = AdamW(params[:of])
+        calls = []
+        monkeypatch.setattr(opt, "step", lambda **kw: calls.append(kw))
+        one = torch.is_tensor(given(params))
+        clip_and_step(opt, given(params), 2.0)
+        fused = (of == 1) == one
+        assert calls == [{"max_norm": 2.0} if fused else {}]
+        norm = (36.0 if one else 72.0) ** 0.5
+        want = 3.0 if fused else 3.0 * 2.0 / (norm + 1e-6)
+        assert torch.allclose(params[0].grad, torch.full((4,), want), rtol=1e-6, atol=0.0)
+
+
 # ---------------------------------------------------------------------------------- the restatement itself
 def test_restatement_is_torch_adamw():
     gen = torch.Generator().manual_seed(0)
